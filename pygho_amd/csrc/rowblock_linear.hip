@@ -405,8 +405,9 @@ struct BnBwdArgs {
   const int32_t* m_dyn;      // non-null: row count read from the device (see RlEpi)
 };
 
+// (f16 at width 128: one wavefront per SIMD -- with scalar f32 instructions only, 256 registers per wavefront spill there)
 template <typename T, int D, int ACT>
-__global__ __launch_bounds__(kBlock, 2) void bn_bwd_linear_kernel(T* __restrict__ gx, T* __restrict__ gpre, const T* __restrict__ pre,
+__global__ __launch_bounds__(kBlock, (std::is_same<T, f16>::value && D == 128) ? 1 : 2) void bn_bwd_linear_kernel(T* __restrict__ gx, T* __restrict__ gpre, const T* __restrict__ pre,
                                                                   const T* __restrict__ gh, const T* __restrict__ wl,
                                                                   const T* __restrict__ addend, float* __restrict__ colsum_ws,
                                                                   BnBwdArgs bn, int64_t m_rows) {
