@@ -28,7 +28,10 @@ FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-ffp-contract=
          "-fno-gpu-rdc", "-DNDEBUG",
          # scalar f32 instructions only: the packed forms hipcc makes of ordinary float code have given wrong results on these cards now
          # and then (hipcc's host pass warns that it does not know the feature: harmless)
-         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+         # an f32 product rounded to f16 is two roundings, as written: the mixed-precision instructions would make one of them, in some
+         # kernels and not in others, and kernels that are bit-identical by construction would differ
+         "-Xclang", "-target-feature", "-Xclang", "-fma-mix-insts"]
 
 
 def _resource_usage(remarks: str, src: str) -> dict:
