@@ -848,6 +848,32 @@ typedef struct pygho_collate_desc {
 size_t pygho_collate_desc_bytes(void);
 int pygho_collate_batch(const void* descs, int64_t n_desc, int64_t n_sel, int64_t max_cols, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Row-wise blocks of an MLP without a batch norm (pygho/honn/utils.py:64-73 LayerNorm, :76-82 activations, :85-142 MLP) with the residual
+ * connection of the layer loop (example/zinc.py:287-290).  f32 / bf16 / f16 rows, any width, any row stride (`*_ld`, in elements; 0 = the same
+ * row for every m), any alignment; 16-byte aligned rows of whole 16-byte vectors are faster.  Parameters are stored in the rows' type or in
+ * f32 (`param_dtype`), statistics and sums are f32, every output is rounded once.
+ *
+ * layer norm:   xh = (x - mean_c x) / sqrt(var_c x + eps) (biased variance),   u = xh * weight + bias,   y = act(u) + residual
+ *   (weight / bias nullable = 1 / 0, residual nullable).  x may be f32 while y is 16-bit (x_dtype).
+ * backward:     du = gy act'(u),  slab sums of (du xh, du[, gx]) per channel,  e = du weight,
+ *               gx = (e - mean_c e - xh mean_c(e xh)) / sqrt(var_c x + eps)
+ *   slabs: pygho_layer_norm_act_bwd_slabs(m) x slab_stride floats at most; *n_slabs (host) says how many the launch writes, each `sums` (2 or
+ *   3) x c floats, to be added by pygho_fold_partials.  m_dev (nullable, device): the true row count below the capacity m_cap; rows behind it
+ *   are neither read nor written, and the slabs are those of a launch over exactly that many rows.
+ * ------------------------------------------------------------------------ */
+enum pygho_row_act { PYGHO_ACT_NONE = 0, PYGHO_ACT_RELU = 1, PYGHO_ACT_SILU = 2, PYGHO_ACT_ELU = 3 };
+int pygho_layer_norm_act(void* y, const void* x, int64_t x_ld, const void* weight, const void* bias, int param_dtype, const void* residual,
+                         int64_t residual_ld, int64_t m, int64_t c, double eps, int act, int dtype, int x_dtype, void* stream);
+int pygho_layer_norm_act_bwd_slabs(int64_t m);
+int pygho_layer_norm_act_bwd(void* gx, float* slabs, int64_t slab_stride, int sums, int* n_slabs, const void* x, int64_t x_ld, const void* gy,
+                             int64_t gy_ld, const void* weight, const void* bias, int param_dtype, int64_t m_cap, const int32_t* m_dev, int64_t c,
+                             double eps, int act, int dtype, int x_dtype, void* stream);
+/* out0[0 .. len0) | out1[0 .. len1) | .. = the columns of n_slabs f32 slabs (slab_stride floats apart, a multiple of 4) added in a fixed order
+ * that trailing slabs of zeros do not change; each output in its own dtype (f32 / bf16 / f16), a null output is skipped. */
+int pygho_fold_partials(void* out0, int64_t len0, int dtype0, void* out1, int64_t len1, int dtype1, void* out2, int64_t len2, int dtype2, void* out3,
+                        int64_t len3, int dtype3, const float* slabs, int64_t n_slabs, int64_t slab_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

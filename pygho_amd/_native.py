@@ -152,6 +152,10 @@ PROTOTYPES = {
     "pygho_khop_emit": (I, [P, P, P, L, P, P, P, P, L, I, P]),
     "pygho_pair_count": (I, [P, P, P, L, P, P, P, P, I, P]),
     "pygho_pair_emit": (I, [P, P, P, L, P, P, L, P, P, P, P, I, P]),
+    "pygho_layer_norm_act": (I, [P, P, L, P, P, I, P, L, L, L, D, I, I, I, P]),
+    "pygho_layer_norm_act_bwd_slabs": (I, [L]),
+    "pygho_layer_norm_act_bwd": (I, [P, P, L, I, P, P, L, P, L, P, P, I, L, P, L, D, I, I, I, P]),
+    "pygho_fold_partials": (I, [P, L, I, P, L, I, P, L, I, P, L, I, P, L, L, P]),
 }
 
 _lib: Optional[ctypes.CDLL] = None

@@ -1,10 +1,11 @@
 """
-Torch-level wrappers over the C ABI, one namespace: the implementation lives in four modules by layer --
+Torch-level wrappers over the C ABI, one namespace: the implementation lives in five modules by layer --
 
     plans.py     int32 / CSR index plans, deferred range checks, integer planner primitives
     segment.py   segment-kernel launches, message plans, autograd Functions of the sparse operators
     masked.py    dense (MaskedTensor) path: masked fill / reduce / broadcast, pair kernels, masked batched contraction
     blocks.py    fused dense steps around the aggregation: BatchNorm + activation, cast arena, row-block Linear, tuple blocks
+    rowops.py    row-wise MLP blocks without a batch norm: LayerNorm, Linear and the two joined, with activation and residual
 
 -- and this module re-exports all of it under the historical name (`from pygho_amd import _ops`).  The modules carry A/B
 switches (`USE_*`, thresholds) that tests and tools flip through this namespace: an assignment `_ops.NAME = value` is forwarded
@@ -14,9 +15,9 @@ there is no CPU path.
 import sys
 import types
 
-from . import blocks, masked, plans, segment
+from . import blocks, masked, plans, rowops, segment
 
-_PARTS = (plans, segment, masked, blocks)
+_PARTS = (plans, segment, masked, blocks, rowops)
 _OWNER = {}
 for _m in _PARTS:
     for _k, _v in vars(_m).items():
