@@ -874,6 +874,30 @@ int pygho_layer_norm_act_bwd(void* gx, float* slabs, int64_t slab_stride, int su
 int pygho_fold_partials(void* out0, int64_t len0, int dtype0, void* out1, int64_t len1, int dtype1, void* out2, int64_t len2, int dtype2, void* out3,
                         int64_t len3, int dtype3, const float* slabs, int64_t n_slabs, int64_t slab_stride, void* stream);
 
+/* Linear maps of those blocks (pygho/honn/utils.py:126-138), any k and n, f32 / bf16 / f16, f32 accumulation:
+ *   pygho_linear_act     y (m, n) = act(z) + residual,   z = x (m, k) . w (n, k)^T + bias;   with `norm`: act(xh g + h) + residual,
+ *                        xh = (z - mean_n z) / sqrt(var_n z + eps), n <= pygho_linear_norm_max().  y_dtype: dtype, or f32 (z unrounded; no
+ *                        norm, no residual)
+ *   pygho_linear_act_dz  dz (m, n) = the gradient of z for the output gradient gy, z formed again from x.  With `norm` also slab sums (g's, h's
+ *                        gradients) of 2 n floats: pygho_linear_act_dz_slabs(m) x slab_stride floats at most, *n_slabs (host) written
+ *   pygho_linear_dx      gx (m, k) = dz . w
+ *   pygho_linear_dw      slabs of dw (n, k) = dz^T . x and, with want_colsum, n column sums of dz behind it: pygho_linear_dw_slabs(m, k, n)
+ *                        slabs, each written
+ * Slabs are added by pygho_fold_partials.  m_dev as for pygho_layer_norm_act_bwd.  Leading dimensions in elements; bias / g / h / residual
+ * nullable (0 / 1 / 0 / 0). */
+int pygho_linear_norm_max(void);
+int pygho_linear_act(void* y, const void* x, int64_t x_ld, const void* w, int64_t w_ld, const void* bias, int bias_dtype, int norm, const void* g,
+                     const void* h, int norm_dtype, double eps, const void* residual, int64_t residual_ld, int64_t m, int64_t k, int64_t n, int act,
+                     int dtype, int y_dtype, void* stream);
+int pygho_linear_act_dz_slabs(int64_t m);
+int pygho_linear_act_dz(void* dz, float* slabs, int64_t slab_stride, int* n_slabs, const void* x, int64_t x_ld, const void* w, int64_t w_ld,
+                        const void* bias, int bias_dtype, int norm, const void* g, const void* h, int norm_dtype, double eps, const void* gy,
+                        int64_t gy_ld, int64_t m_cap, const int32_t* m_dev, int64_t k, int64_t n, int act, int dtype, void* stream);
+int pygho_linear_dx(void* gx, const void* dz, int64_t dz_ld, const void* w, int64_t w_ld, int64_t m, int64_t k, int64_t n, int dtype, void* stream);
+int pygho_linear_dw_slabs(int64_t m, int64_t k, int64_t n);
+int pygho_linear_dw(float* slabs, int64_t slab_stride, const void* dz, int64_t dz_ld, const void* x, int64_t x_ld, int64_t m_cap,
+                    const int32_t* m_dev, int64_t k, int64_t n, int want_colsum, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

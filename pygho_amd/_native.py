@@ -155,6 +155,13 @@ PROTOTYPES = {
     "pygho_layer_norm_act": (I, [P, P, L, P, P, I, P, L, L, L, D, I, I, I, P]),
     "pygho_layer_norm_act_bwd_slabs": (I, [L]),
     "pygho_layer_norm_act_bwd": (I, [P, P, L, I, P, P, L, P, L, P, P, I, L, P, L, D, I, I, I, P]),
+    "pygho_linear_norm_max": (I, []),
+    "pygho_linear_act": (I, [P, P, L, P, L, P, I, I, P, P, I, D, P, L, L, L, L, I, I, I, P]),
+    "pygho_linear_act_dz_slabs": (I, [L]),
+    "pygho_linear_act_dz": (I, [P, P, L, P, P, L, P, L, P, I, I, P, P, I, D, P, L, L, P, L, L, I, I, P]),
+    "pygho_linear_dx": (I, [P, P, L, P, L, L, L, L, I, P]),
+    "pygho_linear_dw_slabs": (I, [L, L, L]),
+    "pygho_linear_dw": (I, [P, L, P, L, P, L, L, P, L, L, I, I, P]),
     "pygho_fold_partials": (I, [P, L, I, P, L, I, P, L, I, P, L, I, P, L, L, P]),
 }
 

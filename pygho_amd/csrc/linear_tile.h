@@ -1,0 +1,471 @@
+// Linear maps of the MLPs with what surrounds them in one launch (reference honn/utils.py:126-138: Linear -> norm -> act; the residual
+// connection of example/zinc.py:287-290), for any width, row stride, alignment, f32 / bf16 / f16:
+//   forward         z = x W^T + b,  y = act(z) + r            or, with a layer norm over the N output channels in between,
+//                   y = act(xh g + h) + r,  xh = (z - mean_n z) / sqrt(var_n z + eps)
+//   gradient of z   z formed again from x (a tile's product costs less than writing z in the forward and reading it back),
+//                   dz = gy act'(z)     or through the norm: du = gy act'(xh g + h), e = du g, dz = rstd (e - mean e - xh mean(e xh))
+//   dX = dz W,      dW = dz^T x  (+ db = the column sums of dz)
+// One tiled product serves all of them.  Output element (m, n) = sum_k P(m, k) Q(n, k); an operand is stored with its k contiguous ("rows": x
+// and W of the forward, dz of dX) or with its m / n contiguous ("columns": W of dX, dz and x of dW).  A step of the k loop moves 128
+// bytes of k per row (64 16-bit or 32 f32 values) global -> registers -> LDS, one step ahead of the matrix instructions.  The MFMA runs in
+// the swapped form D[n][m]: a lane holds one row m and 4 consecutive n, so a row's channels sit in the 4 lanes {m, m + 16, m + 32, m + 48}
+// of ONE wavefront when the tile spans all N: the norm is two lane exchanges per sum, and the epilogue never leaves the registers.
+// Column operands stay in their storage order in LDS; 16-bit fragments are read back transposed by the LDS itself (ds_read_b64_tr_b16),
+// f32 ones element by element (conflict-free, and an f32 MFMA takes 32 cycles).
+// f32 products run on v_mfma_f32_16x16x4f32: true f32, no reduced-precision path.
+#pragma once
+#include "row_ops.h"
+
+namespace pygho {
+
+typedef __attribute__((ext_vector_type(8))) __bf16 la_bf16x8_t;
+typedef __attribute__((ext_vector_type(8))) _Float16 la_f16x8_t;
+typedef __attribute__((ext_vector_type(4))) float la_f32x4_t;
+typedef __attribute__((ext_vector_type(4))) short la_s4_t;
+
+enum { LA_ROWS = 0, LA_COLS = 1 };
+// epilogues: activation (+ residual); norm + activation (+ residual); gradient of z without / with the norm; f32 slab of a split product
+enum { LA_ACT = 0, LA_NORM = 1, LA_DACT = 2, LA_DNORM = 3, LA_SLAB = 4 };
+
+struct LaOperand { const void* p; int64_t ld; int vec; };      // vec: rows on 16-byte boundaries (16-byte loads where they fit)
+
+struct LaArgs {
+  LaOperand a, b;                     // P (m, k), Q (n, k)
+  int64_t m; int64_t n; int64_t k;    // k: of the whole product; LA_SLAB: an upper bound of it (k_dev: the true one)
+  const int32_t* k_dev;
+  void* out; int64_t out_ld; int out_vec; int out_f32;  // out_f32: LA_ACT stores the f32 values as they are
+  const void* bias; int bias_dtype;
+  const void* res; int64_t res_ld; int res_vec;       // forward: the residual; LA_DACT / LA_DNORM: the output gradient
+  const void* g; const void* h; int norm_dtype;
+  float eps; int act;
+  float* slabs; int64_t slab_stride; int splits;      // LA_SLAB: slab s = [m * n product | m column sums (want_sums)]; LA_DNORM: [gg | gh]
+  int want_sums;
+  const int32_t* m_dev;                               // LA_DNORM / LA_DACT: true row count
+};
+
+// one step of k (64 bytes per row): bf16 / f16 one 16x16x32 MFMA, f32 four 16x16x4 (element j of every lane's 4 is k = 4 q + j on both sides)
+template <typename T> __device__ __forceinline__ la_f32x4_t la_mfma(const uint4& a, const uint4& b, la_f32x4_t c) {
+  if constexpr (std::is_same<T, bf16>::value) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(la_bf16x8_t, a), __builtin_bit_cast(la_bf16x8_t, b), c, 0, 0, 0);
+  } else if constexpr (std::is_same<T, f16>::value) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(la_f16x8_t, a), __builtin_bit_cast(la_f16x8_t, b), c, 0, 0, 0);
+  } else {
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.x), __uint_as_float(b.x), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.y), __uint_as_float(b.y), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.z), __uint_as_float(b.z), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.w), __uint_as_float(b.w), c, 0, 0, 0);
+  }
+}
+template <typename T> __device__ __forceinline__ uint4 la_ones() {
+  if constexpr (std::is_same<T, bf16>::value) return make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
+  if constexpr (std::is_same<T, f16>::value) return make_uint4(0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u);
+  return make_uint4(0x3f800000u, 0x3f800000u, 0x3f800000u, 0x3f800000u);
+}
+__device__ __forceinline__ float la_q_sum(float v) {     // over the 4 lanes of a row: q = lane / 16
+  auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+  v = __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+  r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+  return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+}
+
+// geometry of an operand tile of R rows x 128 bytes of k in LDS
+template <typename T, int MODE, int R> struct LaTile {
+  static constexpr int ES = sizeof(T);
+  static constexpr int KE = 128 / ES;                                            // k values per step of the loop
+  // + 16 bytes per row: the 16 rows of a fragment read fall on different banks.  Columns: + 32 (16-bit: the 4 k rows of a transposed read)
+  // or + 16 bytes (f32: the 4 k rows of a wavefront's element reads)
+  static constexpr int PITCH = MODE == LA_ROWS ? 128 + 16 : R * ES + (ES == 2 ? 32 : 16);
+  static constexpr int BYTES = MODE == LA_ROWS ? R * PITCH : KE * PITCH;
+  static constexpr int CHUNKS = R * 8;                                           // 16-byte chunks per step
+  static constexpr int PER_THREAD = (CHUNKS + kBlock - 1) / kBlock;
+  static constexpr int CPR = MODE == LA_ROWS ? 8 : R * ES / 16;                  // chunks per LDS row
+
+  // chunk `i` of this thread: rows [r0, r0 + R) x k [k0, k0 + KE) of the operand; everything outside (n_rows, k_end) is zero
+  static __device__ __forceinline__ uint4 load(const LaOperand& op, int64_t r0, int64_t n_rows, int64_t k0, int64_t k_end, int i) {
+    constexpr int E = 16 / ES;
+    const int c = i * kBlock + (int)threadIdx.x;
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (CHUNKS % kBlock != 0 && c >= CHUNKS) return v;
+    const int lr = c / CPR, lc = c % CPR;
+    const T* base = reinterpret_cast<const T*>(op.p);
+    // `outer` runs over LDS rows, `inner` is the contiguous direction
+    const int64_t outer = MODE == LA_ROWS ? r0 + lr : k0 + lr, outer_end = MODE == LA_ROWS ? n_rows : k_end;
+    const int64_t inner = (MODE == LA_ROWS ? k0 : r0) + lc * E, inner_end = MODE == LA_ROWS ? k_end : n_rows;
+    if (outer >= outer_end || inner >= inner_end) return v;
+    const T* p = base + outer * op.ld + inner;
+    if (op.vec && inner + E <= inner_end) return *reinterpret_cast<const uint4*>(p);
+    const int left = (int)min((int64_t)E, inner_end - inner);
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (ES == 4) {
+        w[j] = j < left ? reinterpret_cast<const uint32_t*>(p)[j] : 0u;
+      } else {
+        const uint32_t lo = 2 * j < left ? reinterpret_cast<const uint16_t*>(p)[2 * j] : 0u;
+        const uint32_t hi = 2 * j + 1 < left ? reinterpret_cast<const uint16_t*>(p)[2 * j + 1] : 0u;
+        w[j] = lo | (hi << 16);
+      }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  static __device__ __forceinline__ void store(char* lds, const uint4& v, int i) {
+    const int c = i * kBlock + (int)threadIdx.x;
+    if (CHUNKS % kBlock != 0 && c >= CHUNKS) return;
+    *reinterpret_cast<uint4*>(lds + (c / CPR) * PITCH + (c % CPR) * 16) = v;
+  }
+  // the lane's 16 bytes of k of row `row0 + lane % 16` in half-step ks (0, 1)
+  static __device__ __forceinline__ uint4 frag(const char* lds, int row0, int ks, int r16, int q) {
+    if constexpr (MODE == LA_ROWS) {
+      return *reinterpret_cast<const uint4*>(lds + (row0 + r16) * PITCH + ks * 64 + q * 16);
+    } else if constexpr (ES == 2) {
+      const char* p = lds + (ks * 32 + q * 8 + (r16 >> 2)) * PITCH + row0 * 2 + (r16 & 3) * 8;
+      const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) la_s4_t*)p));
+      const uint2 hi = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) la_s4_t*)(p + 4 * PITCH)));
+      return make_uint4(lo.x, lo.y, hi.x, hi.y);
+    } else {
+      const char* p = lds + (ks * 16 + q * 4) * PITCH + (row0 + r16) * 4;
+      return make_uint4(*reinterpret_cast<const uint32_t*>(p), *reinterpret_cast<const uint32_t*>(p + PITCH),
+                        *reinterpret_cast<const uint32_t*>(p + 2 * PITCH), *reinterpret_cast<const uint32_t*>(p + 3 * PITCH));
+    }
+  }
+};
+
+constexpr int kLaChunk = 128;         // rows of a split product's reduction per chunk: chunk j belongs to split j % splits
+
+// 4 consecutive elements (of row m, from n) <-> registers; `vec`: the rows are aligned for one access of 4 elements
+template <typename T> __device__ __forceinline__ void la_load4(const T* p, int left, int vec, float (&v)[4]) {
+  if (vec && left >= 4) {
+    if constexpr (sizeof(T) == 4) {
+      const uint4 r = *reinterpret_cast<const uint4*>(p);
+      v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
+    } else {
+      const uint2 r = *reinterpret_cast<const uint2*>(p);
+      float t[8];
+      Vec16<T>::unpack(make_uint4(r.x, r.y, 0u, 0u), t);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = t[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < left ? load_as_acc<T>(p + i) : 0.f;
+  }
+}
+template <typename T> __device__ __forceinline__ void la_store4(T* p, int left, int vec, const float (&v)[4]) {
+  if (vec && left >= 4) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<uint4*>(p) = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    } else {
+      const float t[8] = {v[0], v[1], v[2], v[3], 0.f, 0.f, 0.f, 0.f};
+      const uint4 r = Vec16<T>::pack(t);
+      *reinterpret_cast<uint2*>(p) = make_uint2(r.x, r.y);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) if (i < left) store_from_acc<T>(p + i, v[i]);
+  }
+}
+
+// a workgroup of 4 wavefronts (WM x WN) forms BM x BN output tiles
+template <typename T, int MA, int MB, int BM, int BN, int WM, int WN, int EPI>
+__global__ __launch_bounds__(kBlock) void linear_tile_kernel(LaArgs g) {
+  using TA = LaTile<T, MA, BM>;
+  using TB = LaTile<T, MB, BN>;
+  constexpr int KE = TA::KE, TM = BM / WM, TN = BN / WN, NM = TM / 16, NN = TN / 16;
+  constexpr bool P = Precise<T>::value;
+  static_assert(WM * WN * kWave == kBlock && TM % 16 == 0 && TN % 16 == 0, "tile");
+  static_assert((EPI != LA_NORM && EPI != LA_DNORM) || WN == 1, "a row's channels stay in one wavefront");
+  __shared__ __attribute__((aligned(16))) char lds_a[TA::BYTES];
+  __shared__ __attribute__((aligned(16))) char lds_b[TB::BYTES];
+  const int lane = threadIdx.x & 63, wave = PYGHO_WAVE_INDEX(threadIdx.x >> 6);
+  const int r16 = lane & 15, q = lane >> 4;
+  const int wm = (wave / WN) * TM, wn = (wave % WN) * TN;
+  int64_t m_rows = g.m, k_end = g.k;
+  if constexpr (EPI == LA_DACT || EPI == LA_DNORM) { if (g.m_dev) m_rows = *g.m_dev; }
+  if constexpr (EPI == LA_SLAB) { if (g.k_dev) k_end = *g.k_dev; }
+  const int64_t tiles_n = (g.n + BN - 1) / BN, tiles_m = (m_rows + BM - 1) / BM;
+  const int splits = EPI == LA_SLAB ? g.splits : 1;
+  const int64_t tiles = tiles_m * tiles_n * splits;
+  // consecutive workgroups go to the 8 XCDs in turn: with several column tiles, an XCD takes a contiguous range of tiles (column tile
+  // innermost), so that the row tile they share is read from HBM once and from that XCD's L2 after that
+  const int64_t per_xcd = (tiles + 7) / 8;
+  float sg[EPI == LA_DNORM ? NN : 1][4], sh[EPI == LA_DNORM ? NN : 1][4];
+  if constexpr (EPI == LA_DNORM) {
+#pragma unroll
+    for (int nb = 0; nb < NN; ++nb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { sg[nb][i] = 0.f; sh[nb][i] = 0.f; }
+  }
+
+  for (int64_t slot = blockIdx.x; slot < per_xcd * 8; slot += gridDim.x) {
+    const int64_t t = tiles_n * splits > 1 ? (slot & 7) * per_xcd + (slot >> 3) : slot;
+    if (t >= tiles) continue;
+    const int split = (int)(t % splits);                // (splits of one output tile side by side: they write far apart anyway)
+    const int64_t tt = t / splits;
+    const int64_t m0 = (tt / tiles_n) * BM, n0 = (tt % tiles_n) * BN;
+    // the steps of the reduction: k0(it).  A split walks chunks split, split + splits, ...
+    constexpr int SUB = kLaChunk / KE;
+    int64_t n_it;
+    if constexpr (EPI == LA_SLAB) {
+      const int64_t chunks = (k_end + kLaChunk - 1) / kLaChunk;
+      n_it = chunks > split ? ((chunks - 1 - split) / splits + 1) * SUB : 0;
+    } else {
+      n_it = (k_end + KE - 1) / KE;
+    }
+    auto k_of = [&](int64_t it) -> int64_t {
+      if constexpr (EPI == LA_SLAB) return (split + (it / SUB) * splits) * kLaChunk + (it % SUB) * KE;
+      return it * KE;
+    };
+    uint4 ra[TA::PER_THREAD], rb[TB::PER_THREAD];
+    auto fetch = [&](int64_t k0) {
+#pragma unroll
+      for (int i = 0; i < TA::PER_THREAD; ++i) ra[i] = TA::load(g.a, m0, m_rows, k0, k_end, i);
+#pragma unroll
+      for (int i = 0; i < TB::PER_THREAD; ++i) rb[i] = TB::load(g.b, n0, g.n, k0, k_end, i);
+    };
+    la_f32x4_t acc[NM][NN], ones_acc[EPI == LA_SLAB ? NM : 1];
+#pragma unroll
+    for (int i = 0; i < NM; ++i)
+#pragma unroll
+      for (int j = 0; j < NN; ++j) acc[i][j] = la_f32x4_t{0.f, 0.f, 0.f, 0.f};
+    if constexpr (EPI == LA_SLAB) {
+#pragma unroll
+      for (int i = 0; i < NM; ++i) ones_acc[i] = la_f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    const bool sums = EPI == LA_SLAB && g.want_sums && n0 == 0 && wn == 0;
+    if (n_it > 0) fetch(k_of(0));
+    for (int64_t it = 0; it < n_it; ++it) {
+      __syncthreads();                                   // the previous step's fragments are read
+#pragma unroll
+      for (int i = 0; i < TA::PER_THREAD; ++i) TA::store(lds_a, ra[i], i);
+#pragma unroll
+      for (int i = 0; i < TB::PER_THREAD; ++i) TB::store(lds_b, rb[i], i);
+      __syncthreads();
+      if (it + 1 < n_it) fetch(k_of(it + 1));
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        uint4 fm[NM], fn[NN];
+#pragma unroll
+        for (int i = 0; i < NM; ++i) fm[i] = TA::frag(lds_a, wm + i * 16, ks, r16, q);
+#pragma unroll
+        for (int j = 0; j < NN; ++j) fn[j] = TB::frag(lds_b, wn + j * 16, ks, r16, q);
+#pragma unroll
+        for (int j = 0; j < NN; ++j)
+#pragma unroll
+          for (int i = 0; i < NM; ++i) acc[i][j] = la_mfma<T>(fn[j], fm[i], acc[i][j]);
+        if (sums) {                                      // column sums of dz: the same fragments against ones
+#pragma unroll
+          for (int i = 0; i < NM; ++i) ones_acc[i] = la_mfma<T>(la_ones<T>(), fm[i], ones_acc[i]);
+        }
+      }
+    }
+
+    // ---- epilogue: lane (r16, q) holds rows m0 + wm + 16 i + r16, channels n0 + wn + 16 j + 4 q .. + 3 ----------------------------
+    if constexpr (EPI == LA_SLAB) {
+      float* slab = g.slabs + (int64_t)split * g.slab_stride;
+#pragma unroll
+      for (int i = 0; i < NM; ++i) {
+        const int64_t m = m0 + wm + i * 16 + r16;
+        if (m >= g.m) continue;
+#pragma unroll
+        for (int j = 0; j < NN; ++j) {
+          const int64_t n = n0 + wn + j * 16 + q * 4;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) if (n + e < g.n) slab[m * g.n + n + e] = acc[i][j][e];
+        }
+        if (sums && q == 0) slab[g.m * g.n + m] = ones_acc[i][0];
+      }
+    } else {
+      const T* res = reinterpret_cast<const T*>(g.res);
+      T* out = reinterpret_cast<T*>(g.out);
+#pragma unroll
+      for (int j = 0; j < NN; ++j) {
+        float bv[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int64_t n = n0 + wn + j * 16 + q * 4 + e;
+          bv[e] = n < g.n ? ro_param(g.bias, g.bias_dtype, n, 0.f) : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < NM; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] += bv[e];
+      }
+#pragma unroll
+      for (int i = 0; i < NM; ++i) {
+        const int64_t m = m0 + wm + i * 16 + r16;
+        const bool row_ok = m < m_rows;
+        float rstd = 0.f;
+        if constexpr (EPI == LA_NORM || EPI == LA_DNORM) {
+          // statistics of the row from its registers: mean, then the centred squares; acc becomes xh (absent channels: 0)
+          const float inv_n = 1.f / (float)g.n;
+          float s = 0.f, v = 0.f;
+#pragma unroll
+          for (int j = 0; j < NN; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s += acc[i][j][e];
+          const float mean = la_q_sum(s) * inv_n;
+#pragma unroll
+          for (int j = 0; j < NN; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float d = wn + j * 16 + q * 4 + e < g.n ? acc[i][j][e] - mean : 0.f;
+              acc[i][j][e] = d;
+              v = fmaf(d, d, v);
+            }
+          rstd = 1.f / sqrtf(la_q_sum(v) * inv_n + g.eps);
+#pragma unroll
+          for (int j = 0; j < NN; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][e] *= rstd;
+        }
+        if constexpr (EPI == LA_ACT || EPI == LA_NORM) {
+#pragma unroll
+          for (int j = 0; j < NN; ++j) {
+            const int64_t n = n0 + wn + j * 16 + q * 4;
+            const int left = (int)min((int64_t)4, g.n - n);
+            float u[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+            if constexpr (EPI == LA_NORM) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                u[e] = e < left ? fmaf(u[e], ro_param(g.g, g.norm_dtype, n + e, 1.f), ro_param(g.h, g.norm_dtype, n + e, 0.f)) : 0.f;
+            }
+            ro_act<P, 4>(u, g.act);
+            if (row_ok && left > 0) {
+              if (res) {
+                float r[4];
+                la_load4<T>(res + m * g.res_ld + n, left, g.res_vec, r);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) u[e] += r[e];
+              }
+              if (EPI == LA_ACT && g.out_f32) la_store4<float>(reinterpret_cast<float*>(g.out) + m * g.out_ld + n, left, g.out_vec, u);
+              else la_store4<T>(out + m * g.out_ld + n, left, g.out_vec, u);
+            }
+          }
+        } else {                                         // LA_DACT / LA_DNORM: res = gy
+          float k1 = 0.f, k2 = 0.f;
+          float d[NN][4];
+#pragma unroll
+          for (int j = 0; j < NN; ++j) {
+            const int64_t n = n0 + wn + j * 16 + q * 4;
+            const int left = (int)min((int64_t)4, g.n - n);
+            float z[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]}, w4[4] = {1.f, 1.f, 1.f, 1.f};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[j][e] = 0.f;
+            if (row_ok && left > 0) la_load4<T>(res + m * g.res_ld + n, left, g.res_vec, d[j]);
+            if constexpr (EPI == LA_DNORM) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                w4[e] = e < left ? ro_param(g.g, g.norm_dtype, n + e, 1.f) : 0.f;
+                z[e] = fmaf(z[e], w4[e], e < left ? ro_param(g.h, g.norm_dtype, n + e, 0.f) : 0.f);
+              }
+            }
+            ro_act_slope<P, 4>(d[j], z, g.act);
+            if constexpr (EPI == LA_DNORM) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if (row_ok) {
+                  sg[j][e] = fmaf(d[j][e], acc[i][j][e], sg[j][e]);
+                  sh[j][e] += d[j][e];
+                }
+                d[j][e] *= w4[e];
+                k1 += d[j][e];
+                k2 = fmaf(d[j][e], acc[i][j][e], k2);
+              }
+            }
+          }
+          if constexpr (EPI == LA_DNORM) {
+            const float inv_n = 1.f / (float)g.n;
+            k1 = la_q_sum(k1) * inv_n;
+            k2 = la_q_sum(k2) * inv_n;
+          }
+#pragma unroll
+          for (int j = 0; j < NN; ++j) {
+            const int64_t n = n0 + wn + j * 16 + q * 4;
+            const int left = (int)min((int64_t)4, g.n - n);
+            if constexpr (EPI == LA_DNORM) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) d[j][e] = rstd * (d[j][e] - k1 - acc[i][j][e] * k2);
+            }
+            if (row_ok && left > 0) la_store4<T>(out + m * g.out_ld + n, left, g.out_vec, d[j]);
+          }
+        }
+      }
+    }
+  }
+  if constexpr (EPI == LA_DNORM) {
+    // per-lane sums over the workgroup's rows -> over the 16 lanes of a channel group -> over the wavefronts (LDS, in wave order)
+    float* red = reinterpret_cast<float*>(lds_a);
+    static_assert(TA::BYTES >= WM * BN * 2 * 4, "reduction buffer");
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < NN; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float a = ro_lane_sum<16>(sg[j][e]), b = ro_lane_sum<16>(sh[j][e]);
+        if (r16 == 0) {
+          red[(wave * 2 + 0) * BN + j * 16 + q * 4 + e] = a;
+          red[(wave * 2 + 1) * BN + j * 16 + q * 4 + e] = b;
+        }
+      }
+    __syncthreads();
+    float* slab = g.slabs + (int64_t)blockIdx.x * g.slab_stride;
+    for (int c = threadIdx.x; c < 2 * BN; c += kBlock) {
+      const int s = c / BN, n = c % BN;
+      if (n >= g.n) continue;
+      float a = 0.f;
+      for (int w = 0; w < WM; ++w) a += red[(w * 2 + s) * BN + n];
+      slab[(int64_t)s * g.n + n] = a;
+    }
+  }
+}
+
+static bool la_aligned(const void* p, int64_t ld, int es, int bytes) { return ((uintptr_t)p % bytes) == 0 && (ld * es) % bytes == 0; }
+
+template <typename T, int MA, int MB, int BM, int BN, int WM, int WN, int EPI> static int la_go(const LaArgs& a, int grid_cap, hipStream_t st) {
+  const int64_t tiles = ceil_div(a.m, BM) * ceil_div(a.n, BN) * (EPI == LA_SLAB ? a.splits : 1);
+  const int grid = (int)std::min<int64_t>((tiles + 7) / 8 * 8, grid_cap);
+  hipLaunchKernelGGL((linear_tile_kernel<T, MA, MB, BM, BN, WM, WN, EPI>), dim3(grid), dim3(kBlock), 0, st, a);
+  return check_launch("linear_tile");
+}
+
+constexpr int kLaGrid = 1 << 20;        // workgroups of a launch (a larger product loops)
+
+// Tile of an (m, n) product without a norm: the largest that still gives every CU a workgroup, no wider than the product
+template <typename T, int MA, int MB, int EPI> static int la_any(const LaArgs& a, hipStream_t st) {
+  const int64_t sp = EPI == LA_SLAB ? a.splits : 1;
+  auto count = [&](int bm, int bn) { return ceil_div(a.m, bm) * ceil_div(a.n, bn) * sp; };
+  if (a.n <= 16) return la_go<T, MA, MB, 64, 16, 4, 1, EPI>(a, kLaGrid, st);
+  if (a.n > 64 && a.m > 64 && count(128, 128) >= 256) return la_go<T, MA, MB, 128, 128, 2, 2, EPI>(a, kLaGrid, st);
+  return la_go<T, MA, MB, 64, 64, 2, 2, EPI>(a, kLaGrid, st);
+}
+
+// A norm needs all N channels of a row in one workgroup: N <= 256
+constexpr int kLaNormMax = 256;
+constexpr int kLaNormGrid = 1024;       // LA_DNORM: every workgroup writes a slab
+template <typename T, int EPI> static int la_norm_pick(const LaArgs& a, hipStream_t st, int* slabs) {
+  const int cap = EPI == LA_DNORM ? kLaNormGrid : kLaGrid;
+  // (the gradient's tile does not depend on the row count: a capacity-sized launch must cut the rows as an exactly sized one does)
+  const int bm = a.n > 128 || EPI == LA_DNORM || a.m <= 128 * 256 ? 64 : 128;
+  if (slabs) *slabs = (int)std::min<int64_t>((ceil_div(a.m, bm) + 7) / 8 * 8, cap);
+  if (a.n > 128) return la_go<T, LA_ROWS, LA_ROWS, 64, 256, 4, 1, EPI>(a, cap, st);
+  if (a.n > 64) return bm == 128 ? la_go<T, LA_ROWS, LA_ROWS, 128, 128, 4, 1, EPI>(a, cap, st) : la_go<T, LA_ROWS, LA_ROWS, 64, 128, 4, 1, EPI>(a, cap, st);
+  return bm == 128 ? la_go<T, LA_ROWS, LA_ROWS, 128, 64, 4, 1, EPI>(a, cap, st) : la_go<T, LA_ROWS, LA_ROWS, 64, 64, 4, 1, EPI>(a, cap, st);
+}
+
+// one translation unit per storage type (linear_f32.hip, ..) instantiates these
+template <typename T> int la_forward(const LaArgs& a, int norm, hipStream_t st);
+template <typename T> int la_dz(const LaArgs& a, int norm, hipStream_t st, int* slabs);
+template <typename T> int la_dx(const LaArgs& a, hipStream_t st);
+template <typename T> int la_dw(const LaArgs& a, hipStream_t st);
+
+#define PYGHO_LINEAR_TYPE(T)                                                                                              \
+  template <> int la_forward<T>(const LaArgs& a, int norm, hipStream_t st) {                                              \
+    return norm ? la_norm_pick<T, LA_NORM>(a, st, nullptr) : la_any<T, LA_ROWS, LA_ROWS, LA_ACT>(a, st);                  \
+  }                                                                                                                       \
+  template <> int la_dz<T>(const LaArgs& a, int norm, hipStream_t st, int* slabs) {                                       \
+    return norm ? la_norm_pick<T, LA_DNORM>(a, st, slabs) : la_any<T, LA_ROWS, LA_ROWS, LA_DACT>(a, st);                  \
+  }                                                                                                                       \
+  template <> int la_dx<T>(const LaArgs& a, hipStream_t st) { return la_any<T, LA_ROWS, LA_COLS, LA_ACT>(a, st); }        \
+  template <> int la_dw<T>(const LaArgs& a, hipStream_t st) { return la_any<T, LA_COLS, LA_COLS, LA_SLAB>(a, st); }
+
+}  // namespace pygho

@@ -1,6 +1,7 @@
 // Shared pieces of the row-wise block operators (layer_norm.hip, linear_act.hip): activations and their slopes over register arrays,
 // vectors of a storage type <-> f32 registers, parameters of either storage type, sums over the lanes that share a row.
 #pragma once
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
