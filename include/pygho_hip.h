@@ -854,49 +854,38 @@ int pygho_collate_batch(const void* descs, int64_t n_desc, int64_t n_sel, int64_
  * row for every m), any alignment; 16-byte aligned rows of whole 16-byte vectors are faster.  Parameters are stored in the rows' type or in
  * f32 (`param_dtype`), statistics and sums are f32, every output is rounded once.
  *
+ * m_dev (nullable, device): the true row count of a backward pass below the capacity m_cap; rows behind it are neither read nor written, and the
+ * sums are those of a call over exactly that many rows.  Gradients of parameters are nullable and have their own dtypes; sums over rows are taken
+ * in a fixed order, without atomics.  `workspace`: 16-byte aligned, of the size the *_workspace query returns; nothing in it outlives the call.
+ *
  * layer norm:   xh = (x - mean_c x) / sqrt(var_c x + eps) (biased variance),   u = xh * weight + bias,   y = act(u) + residual
- *   (weight / bias nullable = 1 / 0, residual nullable).  x may be f32 while y is 16-bit (x_dtype).
- * backward:     du = gy act'(u),  slab sums of (du xh, du[, gx]) per channel,  e = du weight,
- *               gx = (e - mean_c e - xh mean_c(e xh)) / sqrt(var_c x + eps)
- *   slabs: pygho_layer_norm_act_bwd_slabs(m) x slab_stride floats at most; *n_slabs (host) says how many the launch writes, each `sums` (2 or
- *   3) x c floats, to be added by pygho_fold_partials.  m_dev (nullable, device): the true row count below the capacity m_cap; rows behind it
- *   are neither read nor written, and the slabs are those of a launch over exactly that many rows.
+ *   (weight / bias nullable = 1 / 0, residual nullable)
+ * backward:     du = gy act'(u),  gweight = sum_m du xh,  gbias = sum_m du,  e = du weight,
+ *               gx = (e - mean_c e - xh mean_c(e xh)) / sqrt(var_c x + eps);   the residual's gradient is gy itself
  * ------------------------------------------------------------------------ */
 enum pygho_row_act { PYGHO_ACT_NONE = 0, PYGHO_ACT_RELU = 1, PYGHO_ACT_SILU = 2, PYGHO_ACT_ELU = 3 };
 int pygho_layer_norm_act(void* y, const void* x, int64_t x_ld, const void* weight, const void* bias, int param_dtype, const void* residual,
-                         int64_t residual_ld, int64_t m, int64_t c, double eps, int act, int dtype, int x_dtype, void* stream);
-int pygho_layer_norm_act_bwd_slabs(int64_t m);
-int pygho_layer_norm_act_bwd(void* gx, float* slabs, int64_t slab_stride, int sums, int* n_slabs, const void* x, int64_t x_ld, const void* gy,
+                         int64_t residual_ld, int64_t m, int64_t c, double eps, int act, int dtype, void* stream);
+size_t pygho_layer_norm_act_bwd_workspace(int64_t m, int64_t c);
+int pygho_layer_norm_act_bwd(void* gx, void* gweight, int gweight_dtype, void* gbias, int gbias_dtype, const void* x, int64_t x_ld, const void* gy,
                              int64_t gy_ld, const void* weight, const void* bias, int param_dtype, int64_t m_cap, const int32_t* m_dev, int64_t c,
-                             double eps, int act, int dtype, int x_dtype, void* stream);
-/* out0[0 .. len0) | out1[0 .. len1) | .. = the columns of n_slabs f32 slabs (slab_stride floats apart, a multiple of 4) added in a fixed order
- * that trailing slabs of zeros do not change; each output in its own dtype (f32 / bf16 / f16), a null output is skipped. */
-int pygho_fold_partials(void* out0, int64_t len0, int dtype0, void* out1, int64_t len1, int dtype1, void* out2, int64_t len2, int dtype2, void* out3,
-                        int64_t len3, int dtype3, const float* slabs, int64_t n_slabs, int64_t slab_stride, void* stream);
+                             double eps, int act, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
-/* Linear maps of those blocks (pygho/honn/utils.py:126-138), any k and n, f32 / bf16 / f16, f32 accumulation:
- *   pygho_linear_act     y (m, n) = act(z) + residual,   z = x (m, k) . w (n, k)^T + bias;   with `norm`: act(xh g + h) + residual,
- *                        xh = (z - mean_n z) / sqrt(var_n z + eps), n <= pygho_linear_norm_max().  y_dtype: dtype, or f32 (z unrounded; no
- *                        norm, no residual)
- *   pygho_linear_act_dz  dz (m, n) = the gradient of z for the output gradient gy, z formed again from x.  With `norm` also slab sums (g's, h's
- *                        gradients) of 2 n floats: pygho_linear_act_dz_slabs(m) x slab_stride floats at most, *n_slabs (host) written
- *   pygho_linear_dx      gx (m, k) = dz . w
- *   pygho_linear_dw      slabs of dw (n, k) = dz^T . x and, with want_colsum, n column sums of dz behind it: pygho_linear_dw_slabs(m, k, n)
- *                        slabs, each written
- * Slabs are added by pygho_fold_partials.  m_dev as for pygho_layer_norm_act_bwd.  Leading dimensions in elements; bias / g / h / residual
- * nullable (0 / 1 / 0 / 0). */
-int pygho_linear_norm_max(void);
-int pygho_linear_act(void* y, const void* x, int64_t x_ld, const void* w, int64_t w_ld, const void* bias, int bias_dtype, int norm, const void* g,
-                     const void* h, int norm_dtype, double eps, const void* residual, int64_t residual_ld, int64_t m, int64_t k, int64_t n, int act,
-                     int dtype, int y_dtype, void* stream);
-int pygho_linear_act_dz_slabs(int64_t m);
-int pygho_linear_act_dz(void* dz, float* slabs, int64_t slab_stride, int* n_slabs, const void* x, int64_t x_ld, const void* w, int64_t w_ld,
-                        const void* bias, int bias_dtype, int norm, const void* g, const void* h, int norm_dtype, double eps, const void* gy,
-                        int64_t gy_ld, int64_t m_cap, const int32_t* m_dev, int64_t k, int64_t n, int act, int dtype, void* stream);
-int pygho_linear_dx(void* gx, const void* dz, int64_t dz_ld, const void* w, int64_t w_ld, int64_t m, int64_t k, int64_t n, int dtype, void* stream);
-int pygho_linear_dw_slabs(int64_t m, int64_t k, int64_t n);
-int pygho_linear_dw(float* slabs, int64_t slab_stride, const void* dz, int64_t dz_ld, const void* x, int64_t x_ld, int64_t m_cap,
-                    const int32_t* m_dev, int64_t k, int64_t n, int want_colsum, int dtype, void* stream);
+/* Linear maps of those blocks (pygho/honn/utils.py:126-138), any k and n:
+ *   z = x (m, k) . w (n, k)^T + bias,    y = act(z) + residual,    with `norm`: y = act(xh g + h) + residual, xh the layer norm of z over n
+ *   (bias / g / h / residual nullable = 0 / 1 / 0 / 0; w in the rows' type).
+ * z: the pre-activation, (m, n).  pygho_linear_act_keeps says whether the backward of this shape reads it: 0 no (z is formed again from x; pass
+ *   NULL), 1 yes, in the rows' type (NULL in a forward that no backward follows), 2 yes, in f32 (the forward itself needs the buffer).
+ * backward: dz = the gradient of z,   gx = dz . w (nullable),   gw = dz^T . x,   gb = sum_m dz,   gg / gh as gweight / gbias above. */
+int pygho_linear_act_keeps(int64_t k, int64_t n, int norm, int act, int dtype);
+int pygho_linear_act(void* y, void* z, const void* x, int64_t x_ld, const void* w, int64_t w_ld, const void* bias, int bias_dtype, int norm,
+                     const void* g, const void* h, int norm_dtype, double eps, const void* residual, int64_t residual_ld, int64_t m, int64_t k,
+                     int64_t n, int act, int dtype, void* stream);
+size_t pygho_linear_act_bwd_workspace(int64_t m, int64_t k, int64_t n, int norm, int act, int dtype);
+int pygho_linear_act_bwd(void* gx, void* gw, int gw_dtype, void* gb, int gb_dtype, void* gg, int gg_dtype, void* gh, int gh_dtype, const void* z,
+                         const void* x, int64_t x_ld, const void* w, int64_t w_ld, const void* bias, int bias_dtype, int norm, const void* g,
+                         const void* h, int norm_dtype, double eps, const void* gy, int64_t gy_ld, int64_t m_cap, const int32_t* m_dev, int64_t k,
+                         int64_t n, int act, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

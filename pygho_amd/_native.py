@@ -152,17 +152,13 @@ PROTOTYPES = {
     "pygho_khop_emit": (I, [P, P, P, L, P, P, P, P, L, I, P]),
     "pygho_pair_count": (I, [P, P, P, L, P, P, P, P, I, P]),
     "pygho_pair_emit": (I, [P, P, P, L, P, P, L, P, P, P, P, I, P]),
-    "pygho_layer_norm_act": (I, [P, P, L, P, P, I, P, L, L, L, D, I, I, I, P]),
-    "pygho_layer_norm_act_bwd_slabs": (I, [L]),
-    "pygho_layer_norm_act_bwd": (I, [P, P, L, I, P, P, L, P, L, P, P, I, L, P, L, D, I, I, I, P]),
-    "pygho_linear_norm_max": (I, []),
-    "pygho_linear_act": (I, [P, P, L, P, L, P, I, I, P, P, I, D, P, L, L, L, L, I, I, I, P]),
-    "pygho_linear_act_dz_slabs": (I, [L]),
-    "pygho_linear_act_dz": (I, [P, P, L, P, P, L, P, L, P, I, I, P, P, I, D, P, L, L, P, L, L, I, I, P]),
-    "pygho_linear_dx": (I, [P, P, L, P, L, L, L, L, I, P]),
-    "pygho_linear_dw_slabs": (I, [L, L, L]),
-    "pygho_linear_dw": (I, [P, L, P, L, P, L, L, P, L, L, I, I, P]),
-    "pygho_fold_partials": (I, [P, L, I, P, L, I, P, L, I, P, L, I, P, L, L, P]),
+    "pygho_layer_norm_act": (I, [P, P, L, P, P, I, P, L, L, L, D, I, I, P]),
+    "pygho_layer_norm_act_bwd_workspace": (Z, [L, L]),
+    "pygho_layer_norm_act_bwd": (I, [P, P, I, P, I, P, L, P, L, P, P, I, L, P, L, D, I, I, P, Z, P]),
+    "pygho_linear_act_keeps": (I, [L, L, I, I, I]),
+    "pygho_linear_act": (I, [P, P, P, L, P, L, P, I, I, P, P, I, D, P, L, L, L, L, I, I, P]),
+    "pygho_linear_act_bwd_workspace": (Z, [L, L, L, I, I, I]),
+    "pygho_linear_act_bwd": (I, [P, P, I, P, I, P, I, P, I, P, P, L, P, L, P, I, I, P, P, I, D, P, L, L, P, L, L, I, I, P, Z, P]),
 }
 
 _lib: Optional[ctypes.CDLL] = None

@@ -6,7 +6,7 @@
 // A row lives in the registers of LPR lanes (NV vectors of VE elements each): the mean, the centred sum of squares (two passes over
 // registers: no cancellation, however far the mean is from zero) and the two sums of the backward are lane-group sums.  The backward
 // takes the statistics from x again instead of loading them: the row is in registers anyway.
-// gg / gh: a lane keeps its channels' sums over all rows of its workgroup; workgroups write one slab each, pygho_fold_partials adds the
+// gg / gh: a lane keeps its channels' sums over all rows of its workgroup; workgroups write one slab each, a second launch adds the
 // slabs in a fixed order.  Chunk k of the rows belongs to workgroup k % grid, so a slab depends on the true rows only: a launch sized for a
 // capacity (m_dev: the count is on the device) gives the bits of an exactly sized one.
 #include "row_ops.h"
@@ -96,7 +96,8 @@ __global__ __launch_bounds__(kBlock) void ln_fwd_kernel(T* __restrict__ y, const
   }
 }
 
-// NS = 2: slabs of (gg, gh); 3: (gg, gh, column sums of gx before their rounding: the bias gradient of a Linear in front of the norm)
+// NS = 2: slabs of (gg, gh); 3: (gg, gh, column sums of gx before their rounding: the bias gradient of a Linear in front of the norm);
+// 1: no norm, gx = gy act'(x) and the column sums of gx (the gradient of a Linear's kept pre-activation)
 template <typename T, typename TX, int VE, int LPR, int NV, int U, int NS>
 __global__ __launch_bounds__(kBlock) void ln_bwd_kernel(T* __restrict__ gx, float* __restrict__ slabs, int64_t slab_stride, const TX* __restrict__ x,
                                                         int64_t x_ld, const T* __restrict__ gy, int64_t gy_ld, const void* __restrict__ w,
@@ -145,6 +146,16 @@ __global__ __launch_bounds__(kBlock) void ln_bwd_kernel(T* __restrict__ gx, floa
     for (int u = 0; u < U; ++u) {
       const bool valid = row[u] < m;
       float rstd, s1 = 0.f, s2 = 0.f;
+      if constexpr (NS == 1) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          ro_act_slope<P, VE>(gv[u][v], xv[u][v], act);
+#pragma unroll
+          for (int j = 0; j < VE; ++j) acc[0][v][j] += valid ? gv[u][v][j] : 0.f;
+          if (on[v] && valid) ro_store<T, VE>(gx + row[u] * c + (v * LPR + lr) * VE, gv[u][v]);
+        }
+        continue;
+      }
       ln_stats<LPR, NV, VE>(xv[u], on, inv_c, eps, rstd);
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
@@ -158,7 +169,7 @@ __global__ __launch_bounds__(kBlock) void ln_bwd_kernel(T* __restrict__ gx, floa
         for (int j = 0; j < VE; ++j) {
           if (valid) {                                     // (a row past the end repeats the last one: it must not count twice)
             acc[0][v][j] = fmaf(gv[u][v][j], xv[u][v][j], acc[0][v][j]);
-            acc[1][v][j] += gv[u][v][j];
+            acc[NS > 1 ? 1 : 0][v][j] += gv[u][v][j];
           }
           gv[u][v][j] *= g[v][j];
           s1 += gv[u][v][j];
@@ -258,6 +269,18 @@ __global__ __launch_bounds__(kBlock) void ln_bwd_wide_kernel(T* __restrict__ gx,
   for (int64_t row = blockIdx.x; row < m; row += gridDim.x, first = false) {
     const TX* xr = x + row * x_ld;
     const T* gr = gy + row * gy_ld;
+    if constexpr (NS == 1) {
+      for (int64_t col = (int64_t)threadIdx.x * VE; col < c; col += kBlock * VE) {
+        float z[VE], t[VE];
+        ro_load<TX, VE>(xr + col, z);
+        ro_load<T, VE>(gr + col, t);
+        ro_act_slope<Precise<T>::value, VE>(t, z, act);
+#pragma unroll
+        for (int j = 0; j < VE; ++j) slab[col + j] = (first ? 0.f : slab[col + j]) + t[j];
+        ro_store<T, VE>(gx + row * c + col, t);
+      }
+      continue;
+    }
     float mean, rstd, s1 = 0.f, s2 = 0.f, xh[VE], d[VE];
     ln_wide_stats<T, TX, VE>(xr, c, eps, lds, mean, rstd);
     auto load_du = [&](int64_t col) {
@@ -305,7 +328,6 @@ __global__ __launch_bounds__(kBlock) void ln_bwd_wide_kernel(T* __restrict__ gx,
 // ---- slabs -> sums in a fixed order: 4 lanes x 4 columns by 64 slab lanes, lane t adds slabs t, t + 64, .., the 64 lanes a tree.  The order
 // does not depend on the slab count, so trailing slabs of zeros change nothing.  64 slab lanes: a fold of a few hundred columns is a
 // handful of workgroups, and with 16 the serial loads of one lane took longer than everything else --------------------------------
-struct FoldOut { void* p[4]; int64_t len[4]; int dt[4]; };
 __global__ __launch_bounds__(kBlock) void fold_partials_kernel(FoldOut out, const float* __restrict__ slabs, int64_t n_slabs, int64_t stride,
                                                                int64_t width) {
   __shared__ float4 red[64][4];
@@ -446,7 +468,7 @@ template <typename T, typename TX, int NS> static int ln_bwd_typed(const LnBwd& 
   return check_launch("layer_norm_act_bwd");
 }
 
-static bool ro_float(int dtype) { return dtype == PYGHO_F32 || dtype == PYGHO_BF16 || dtype == PYGHO_F16; }
+bool ro_float(int dtype) { return dtype == PYGHO_F32 || dtype == PYGHO_BF16 || dtype == PYGHO_F16; }
 
 }  // namespace pygho
 
@@ -465,49 +487,71 @@ static int ln_check(const char* what, const void* a, const void* b, int64_t m, i
 }
 
 extern "C" int pygho_layer_norm_act(void* y, const void* x, int64_t x_ld, const void* weight, const void* bias, int param_dtype, const void* residual,
-                                    int64_t residual_ld, int64_t m, int64_t c, double eps, int act, int dtype, int x_dtype, void* stream) {
-  if (int rc = ln_check("layer_norm_act", y, x, m, c, eps, act, dtype, x_dtype, param_dtype)) return rc;
+                                    int64_t residual_ld, int64_t m, int64_t c, double eps, int act, int dtype, void* stream) {
+  if (int rc = ln_check("layer_norm_act", y, x, m, c, eps, act, dtype, dtype, param_dtype)) return rc;
   if (m == 0) return PYGHO_OK;
-  const LnFwd a{y, x, x_ld, weight, bias, param_dtype, residual, residual_ld, m, c, (float)eps, act, (hipStream_t)stream};
+  return ln_fwd_launch(y, x, x_ld, weight, bias, param_dtype, residual, residual_ld, m, c, (float)eps, act, dtype, dtype, (hipStream_t)stream);
+}
+
+int pygho::ln_fwd_launch(void* y, const void* x, int64_t x_ld, const void* weight, const void* bias, int param_dtype, const void* residual,
+                         int64_t residual_ld, int64_t m, int64_t c, float eps, int act, int dtype, int x_dtype, hipStream_t st) {
+  const LnFwd a{y, x, x_ld, weight, bias, param_dtype, residual, residual_ld, m, c, eps, act, st};
   if (dtype == PYGHO_F32) return ln_fwd_typed<float, float>(a);
   if (dtype == PYGHO_BF16) return x_dtype == PYGHO_F32 ? ln_fwd_typed<bf16, float>(a) : ln_fwd_typed<bf16, bf16>(a);
   return x_dtype == PYGHO_F32 ? ln_fwd_typed<f16, float>(a) : ln_fwd_typed<f16, f16>(a);
 }
 
-extern "C" int pygho_layer_norm_act_bwd_slabs(int64_t m) { return m <= 0 ? 0 : grid_for(m, 1, kLnBwdGrid); }
+// ---- backward: rows and slabs in one launch, the fold in a second; both on the caller's workspace ------------------------------------
+namespace pygho {
 
-extern "C" int pygho_layer_norm_act_bwd(void* gx, float* slabs, int64_t slab_stride, int sums, int* n_slabs, const void* x,
-                                        int64_t x_ld, const void* gy, int64_t gy_ld, const void* weight, const void* bias, int param_dtype, int64_t m_cap, const int32_t* m_dev,
-                                        int64_t c, double eps, int act, int dtype, int x_dtype, void* stream) {
-  if (int rc = ln_check("layer_norm_act_bwd", gx, x, m_cap, c, eps, act, dtype, x_dtype, param_dtype)) return rc;
-  if (!n_slabs) { set_error("null pointer"); return PYGHO_ERR_INVALID; }
-  *n_slabs = 0;
-  if (m_cap == 0) return PYGHO_OK;
-  if (!gy || !slabs) { set_error("null pointer"); return PYGHO_ERR_INVALID; }
-  if ((sums != 2 && sums != 3) || slab_stride < sums * c) { set_error("layer_norm_act_bwd: 2 or 3 sums of c floats per slab"); return PYGHO_ERR_INVALID; }
-  const LnBwd a{gx, slabs, slab_stride, n_slabs, x, x_ld, gy, gy_ld, weight, bias, param_dtype, m_cap, m_dev, c,
-                (float)eps, act, (hipStream_t)stream};
-#define PYGHO_LNB(T, TX) (sums == 3 ? ln_bwd_typed<T, TX, 3>(a) : ln_bwd_typed<T, TX, 2>(a))
+int64_t ln_bwd_slab_floats(int64_t m, int64_t c, int sums) {
+  return m <= 0 ? 0 : (int64_t)grid_for(m, 1, kLnBwdGrid) * ((sums * c + 3) / 4 * 4);
+}
+
+int ln_bwd_launch(void* gx, float* slabs, int64_t* stride, int* n_slabs, int sums, const void* x, int64_t x_ld, const void* gy, int64_t gy_ld,
+                  const void* weight, const void* bias, int param_dtype, int64_t m, const int32_t* m_dev, int64_t c, float eps, int act, int dtype,
+                  int x_dtype, hipStream_t st) {
+  *stride = (sums * c + 3) / 4 * 4;
+  const LnBwd a{gx, slabs, *stride, n_slabs, x, x_ld, gy, gy_ld, weight, bias, param_dtype, m, m_dev, c, eps, act, st};
+#define PYGHO_LNB(T, TX) (sums == 3 ? ln_bwd_typed<T, TX, 3>(a) : sums == 2 ? ln_bwd_typed<T, TX, 2>(a) : ln_bwd_typed<T, TX, 1>(a))
   if (dtype == PYGHO_F32) return PYGHO_LNB(float, float);
   if (dtype == PYGHO_BF16) return x_dtype == PYGHO_F32 ? PYGHO_LNB(bf16, float) : PYGHO_LNB(bf16, bf16);
   return x_dtype == PYGHO_F32 ? PYGHO_LNB(f16, float) : PYGHO_LNB(f16, f16);
 #undef PYGHO_LNB
 }
 
-extern "C" int pygho_fold_partials(void* out0, int64_t len0, int dtype0, void* out1, int64_t len1, int dtype1, void* out2, int64_t len2, int dtype2,
-                                   void* out3, int64_t len3, int dtype3, const float* slabs, int64_t n_slabs, int64_t slab_stride, void* stream) {
-  const FoldOut o{{out0, out1, out2, out3}, {len0, len1, len2, len3}, {dtype0, dtype1, dtype2, dtype3}};
+int fold_launch(const FoldOut& o, const float* slabs, int64_t n_slabs, int64_t stride, hipStream_t st) {
   int64_t width = 0;
-  for (int k = 0; k < 4; ++k) {
-    if (o.len[k] < 0 || (o.len[k] > 0 && o.p[k] && !ro_float(o.dt[k]))) { set_error("fold_partials: bad length or dtype"); return PYGHO_ERR_INVALID; }
-    width += o.len[k];
-  }
-  if (n_slabs < 0 || slab_stride < width || slab_stride % 4 != 0) { set_error("fold_partials: slab_stride >= the summed lengths, a multiple of 4"); return PYGHO_ERR_INVALID; }
+  for (int k = 0; k < 4; ++k) width += o.len[k];
   if (width == 0) return PYGHO_OK;
-  if (n_slabs > 0 && !slabs) { set_error("null pointer"); return PYGHO_ERR_INVALID; }
-  if ((uintptr_t)slabs % 16 != 0) { set_error("fold_partials: slabs must be 16-byte aligned"); return PYGHO_ERR_INVALID; }
   const int64_t grid = ceil_div(width, 16);
   if (grid > INT32_MAX) { set_error("fold_partials: too wide"); return PYGHO_ERR_UNSUPPORTED; }
-  hipLaunchKernelGGL(fold_partials_kernel, dim3((unsigned)grid), dim3(kBlock), 0, (hipStream_t)stream, o, slabs, n_slabs, slab_stride, width);
+  hipLaunchKernelGGL(fold_partials_kernel, dim3((unsigned)grid), dim3(kBlock), 0, st, o, slabs, n_slabs, stride, width);
   return check_launch("fold_partials");
+}
+
+}  // namespace pygho
+
+extern "C" size_t pygho_layer_norm_act_bwd_workspace(int64_t m, int64_t c) { return m <= 0 || c <= 0 ? 0 : (size_t)ln_bwd_slab_floats(m, c, 2) * 4; }
+
+extern "C" int pygho_layer_norm_act_bwd(void* gx, void* gweight, int gweight_dtype, void* gbias, int gbias_dtype, const void* x, int64_t x_ld,
+                                        const void* gy, int64_t gy_ld, const void* weight, const void* bias, int param_dtype, int64_t m_cap,
+                                        const int32_t* m_dev, int64_t c, double eps, int act, int dtype, void* workspace, size_t workspace_bytes,
+                                        void* stream) {
+  if (int rc = ln_check("layer_norm_act_bwd", gx, x, m_cap, c, eps, act, dtype, dtype, param_dtype)) return rc;
+  if ((gweight && !ro_float(gweight_dtype)) || (gbias && !ro_float(gbias_dtype))) { set_error("layer_norm_act_bwd: gradient dtype"); return PYGHO_ERR_UNSUPPORTED; }
+  if (m_cap > 0 && (!gy || !workspace)) { set_error("null pointer"); return PYGHO_ERR_INVALID; }
+  if (workspace_bytes < pygho_layer_norm_act_bwd_workspace(m_cap, c) || (uintptr_t)workspace % 16 != 0) {
+    set_error("layer_norm_act_bwd: workspace too small or not 16-byte aligned");
+    return PYGHO_ERR_INVALID;
+  }
+  hipStream_t st = (hipStream_t)stream;
+  float* slabs = reinterpret_cast<float*>(workspace);
+  int64_t stride = (2 * c + 3) / 4 * 4;
+  int n = 0;
+  if (m_cap > 0) {
+    if (int rc = ln_bwd_launch(gx, slabs, &stride, &n, 2, x, x_ld, gy, gy_ld, weight, bias, param_dtype, m_cap, m_dev, c, (float)eps, act, dtype, dtype, st)) return rc;
+  }
+  if (!gweight && !gbias) return PYGHO_OK;
+  return fold_launch(FoldOut{{gweight, gbias, nullptr, nullptr}, {c, c, 0, 0}, {gweight_dtype, gbias_dtype, 0, 0}}, slabs, n, stride, st);
 }

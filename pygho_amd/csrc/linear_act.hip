@@ -1,120 +1,227 @@
-// Entry points of the linear operators (kernels and their reasons: linear_tile.h): argument checks, operand alignment, type dispatch.
-#include "linear_tile.h"
+// Entry points of the linear operators: argument checks, which form runs (linear_stream.h, linear_tile.h), the launches of a backward pass.
+#include "linear_ops.h"
 
 namespace pygho {
 
-template <> int la_forward<float>(const LaArgs&, int, hipStream_t);
-template <> int la_forward<bf16>(const LaArgs&, int, hipStream_t);
-template <> int la_forward<f16>(const LaArgs&, int, hipStream_t);
-template <> int la_dz<float>(const LaArgs&, int, hipStream_t, int*);
-template <> int la_dz<bf16>(const LaArgs&, int, hipStream_t, int*);
-template <> int la_dz<f16>(const LaArgs&, int, hipStream_t, int*);
-template <> int la_dx<float>(const LaArgs&, hipStream_t);
-template <> int la_dx<bf16>(const LaArgs&, hipStream_t);
-template <> int la_dx<f16>(const LaArgs&, hipStream_t);
-template <> int la_dw<float>(const LaArgs&, hipStream_t);
-template <> int la_dw<bf16>(const LaArgs&, hipStream_t);
-template <> int la_dw<f16>(const LaArgs&, hipStream_t);
+#define PYGHO_LINEAR_DECL(T)                                                                  \
+  template <> bool LinearOps<T>::stream_fits(int64_t, int64_t, int);                          \
+  template <> bool LinearOps<T>::stream_dx_fits(int64_t, int64_t, int);                       \
+  template <> int LinearOps<T>::stream_fwd(const LsArgs&, int, hipStream_t);                  \
+  template <> int LinearOps<T>::stream_bwd(const LsArgs&, int, int*, hipStream_t);            \
+  template <> int LinearOps<T>::tile_act(const LaArgs&, hipStream_t);                         \
+  template <> int LinearOps<T>::tile_dx(const LaArgs&, hipStream_t);                          \
+  template <> int LinearOps<T>::tile_dw(const LaArgs&, hipStream_t);
+PYGHO_LINEAR_DECL(float)
+PYGHO_LINEAR_DECL(bf16)
+PYGHO_LINEAR_DECL(f16)
+#undef PYGHO_LINEAR_DECL
 
-static bool la_float(int d) { return d == PYGHO_F32 || d == PYGHO_BF16 || d == PYGHO_F16; }
-static int la_check(const char* what, int64_t m, int64_t k, int64_t n, int act, int dtype) {
-  if (m < 0 || k <= 0 || n <= 0 || k > INT32_MAX / 2 || n > INT32_MAX / 2) { set_error("%s: bad size", what); return PYGHO_ERR_INVALID; }
-  if (!la_float(dtype)) { set_error("%s: f32 / bf16 / f16 only", what); return PYGHO_ERR_UNSUPPORTED; }
+// f(LinearOps<T>{}) for the storage type
+template <typename F> static auto la_type(int dtype, F&& f) {
+  if (dtype == PYGHO_F32) return f(LinearOps<float>{});
+  if (dtype == PYGHO_BF16) return f(LinearOps<bf16>{});
+  return f(LinearOps<f16>{});
+}
+static int la_size(int dtype) { return dtype == PYGHO_F32 ? 4 : 2; }
+
+static int la_check(const char* what, int64_t m, int64_t k, int64_t n, double eps, int act, int dtype) {
+  if (m < 0 || k <= 0 || n <= 0 || k >= (1 << 26) || n >= (1 << 26)) { set_error("%s: bad size", what); return PYGHO_ERR_INVALID; }
+  if (!ro_float(dtype)) { set_error("%s: f32 / bf16 / f16 only", what); return PYGHO_ERR_UNSUPPORTED; }
   if (act < 0 || act > kActElu) { set_error("%s: unknown activation %d", what, act); return PYGHO_ERR_INVALID; }
+  if (!(eps >= 0.0)) { set_error("%s: eps must not be negative", what); return PYGHO_ERR_INVALID; }
   return PYGHO_OK;
 }
-static LaOperand la_operand(const void* p, int64_t ld, int dtype) {
-  return LaOperand{p, ld, la_aligned(p, ld, dtype == PYGHO_F32 ? 4 : 2, 16) ? 1 : 0};
+static int la_param_check(const char* what, const void* p, int pdt, int dtype) {
+  if (p && pdt != dtype && pdt != PYGHO_F32) { set_error("%s: parameters in the rows' type or in f32", what); return PYGHO_ERR_UNSUPPORTED; }
+  return PYGHO_OK;
+}
+static int la_stride_check(const char* what, int64_t a, int64_t b, int dtype) {        // 32-bit offsets inside a block of 16 rows
+  if (a < 0 || b < 0 || std::max(a, b) * la_size(dtype) >= (1 << 28)) { set_error("%s: row strides of 0 .. 2^28 bytes", what); return PYGHO_ERR_UNSUPPORTED; }
+  return PYGHO_OK;
+}
+static LaOperand la_operand(const void* p, int64_t ld, int dtype) { return LaOperand{p, ld, la_aligned(p, ld, la_size(dtype), 16) ? 1 : 0}; }
+
+// the form of an operator over (k, n): W in LDS, or tiles
+static bool la_streams(int64_t k, int64_t n, int norm, int dtype) {
+  return la_type(dtype, [&](auto ops) { return ops.stream_fits(k, n, norm); });
+}
+static LsArgs la_stream_args(const void* x, int64_t x_ld, const void* w, int64_t w_ld, const void* bias, int bias_dtype, const void* g, const void* h,
+                             int norm_dtype, const void* r, int64_t r_ld, void* out, int64_t m, int64_t k, int64_t n, double eps, int act, int dtype) {
+  const int es = la_size(dtype);
+  LsArgs a{};
+  a.x = x; a.x_ld = x_ld;
+  a.w = w; a.w_ld = w_ld; a.w_vec = la_aligned(w, w_ld, es, 16);
+  a.bias = bias; a.bias_dtype = bias_dtype; a.g = g; a.h = h; a.norm_dtype = norm_dtype;
+  a.r = r; a.r_ld = r_ld;
+  a.out = out;
+  a.vec = k % (64 / es) == 0 && n % 16 == 0 && la_aligned(x, x_ld, es, 16) && la_aligned(r, r_ld, es, 4 * es) && la_aligned(out, n, es, 4 * es);
+  a.m = m; a.k = (int)k; a.n = (int)n; a.eps = (float)eps; a.act = act;
+  return a;
+}
+static int la_tile_act(const void* x, int64_t x_ld, const void* w, int64_t w_ld, const void* bias, int bias_dtype, const void* residual, int64_t residual_ld,
+                       void* y, void* z, int z_f32, int64_t m, int64_t k, int64_t n, int act, int dtype, hipStream_t st) {
+  const int es = la_size(dtype);
+  LaArgs a{};
+  a.a = la_operand(x, x_ld, dtype);
+  a.b = la_operand(w, w_ld, dtype);
+  a.m = m; a.n = n; a.k = k;
+  a.out = y; a.out_vec = la_aligned(y, n, es, 4 * es);
+  a.z = z; a.z_f32 = z_f32; a.z_vec = la_aligned(z, n, z_f32 ? 4 : es, 4 * (z_f32 ? 4 : es));
+  a.bias = bias; a.bias_dtype = bias_dtype;
+  a.res = residual; a.res_ld = residual_ld; a.res_vec = la_aligned(residual, residual_ld, es, 4 * es);
+  a.act = act;
+  return la_type(dtype, [&](auto ops) { return ops.tile_act(a, st); });
+}
+
+// slabs of a weight gradient: enough workgroups for two per CU, at most one per chunk of rows
+static int64_t la_dw_slabs(int64_t m, int64_t k, int64_t n) {
+  if (m <= 0) return 0;
+  const int64_t tiles = (n > 64 && k > 64) ? ceil_div(n, 128) * ceil_div(k, 128) : ceil_div(n, 64) * ceil_div(k, k <= 16 ? 16 : 64);
+  return std::min<int64_t>(ceil_div(m, kLaChunk), std::max<int64_t>(1, 512 / tiles));
+}
+static int64_t la_pad4(int64_t v) { return (v + 3) / 4 * 4; }
+
+// workspace of a backward pass, in bytes: [dz (16-byte padded)] [z] [slabs of the sums over n] [slabs of dW | db].
+// z: a forward that streams has not kept the pre-activation; where its backward is too wide to stream, z is formed again in f32 for the row kernel
+struct LaSpace { int64_t dz, z, sums, dw, total; int nsum; bool stream, own_dz; };
+static LaSpace la_space(int64_t m, int64_t k, int64_t n, int norm, int act, int dtype) {
+  LaSpace s{};
+  const bool fwd_streams = la_streams(k, n, norm, dtype);
+  s.stream = fwd_streams && n <= ls_bwd_max(norm);
+  s.nsum = norm ? 3 : 1;
+  s.own_dz = norm || act != kActNone;
+  s.dz = s.own_dz ? (m * n * la_size(dtype) + 15) / 16 * 16 : 0;
+  s.z = s.own_dz && fwd_streams && !s.stream ? (m * n * 4 + 15) / 16 * 16 : 0;
+  s.sums = !s.own_dz ? 0 : s.stream ? kLsGrid * la_pad4(s.nsum * n) * 4 : ln_bwd_slab_floats(m, n, s.nsum) * 4;
+  s.dw = la_dw_slabs(m, k, n) * la_pad4(n * k + n) * 4;
+  s.total = s.dz + s.z + s.sums + s.dw;
+  return s;
 }
 
 }  // namespace pygho
 
 using namespace pygho;
 
-extern "C" int pygho_linear_norm_max(void) { return kLaNormMax; }
+// what the forward keeps for the backward besides x: 0 nothing, 1 the pre-activation in the rows' type, 2 the pre-activation in f32 (needed by the
+// forward itself as well)
+extern "C" int pygho_linear_act_keeps(int64_t k, int64_t n, int norm, int act, int dtype) {
+  if (k <= 0 || n <= 0 || !ro_float(dtype) || la_streams(k, n, norm, dtype)) return 0;
+  return norm ? 2 : act != kActNone ? 1 : 0;
+}
 
-extern "C" int pygho_linear_act(void* y, const void* x, int64_t x_ld, const void* w, int64_t w_ld, const void* bias, int bias_dtype, int norm,
+extern "C" int pygho_linear_act(void* y, void* z, const void* x, int64_t x_ld, const void* w, int64_t w_ld, const void* bias, int bias_dtype, int norm,
                                 const void* g, const void* h, int norm_dtype, double eps, const void* residual, int64_t residual_ld, int64_t m,
-                                int64_t k, int64_t n, int act, int dtype, int y_dtype, void* stream) {
-  if (int rc = la_check("linear_act", m, k, n, act, dtype)) return rc;
-  if (y_dtype != dtype && (y_dtype != PYGHO_F32 || norm || residual)) { set_error("linear_act: an f32 output has no norm and no residual"); return PYGHO_ERR_UNSUPPORTED; }
-  if (norm && (n > kLaNormMax || !(eps >= 0.0))) { set_error("linear_act: a norm over at most %d channels, eps >= 0", kLaNormMax); return PYGHO_ERR_UNSUPPORTED; }
+                                int64_t k, int64_t n, int act, int dtype, void* stream) {
+  if (int rc = la_check("linear_act", m, k, n, eps, act, dtype)) return rc;
+  if (int rc = la_param_check("linear_act", bias, bias_dtype, dtype)) return rc;
+  if (g || h) { if (int rc = la_param_check("linear_act", g ? g : h, norm_dtype, dtype)) return rc; }
+  if (int rc = la_stride_check("linear_act", x_ld, residual ? residual_ld : 0, dtype)) return rc;
   if (m == 0) return PYGHO_OK;
   if (!y || !x || !w) { set_error("null pointer"); return PYGHO_ERR_INVALID; }
-  const int es = dtype == PYGHO_F32 ? 4 : 2;
-  LaArgs a{};
-  a.a = la_operand(x, x_ld, dtype);
-  a.b = la_operand(w, w_ld, dtype);
-  a.m = m; a.n = n; a.k = k;
-  a.out_f32 = y_dtype == PYGHO_F32;
-  a.out = y; a.out_ld = n; a.out_vec = la_aligned(y, n, a.out_f32 ? 4 : es, 4 * (a.out_f32 ? 4 : es));
-  a.bias = bias; a.bias_dtype = bias_dtype;
-  a.res = residual; a.res_ld = residual_ld; a.res_vec = la_aligned(residual, residual_ld, es, 4 * es);
-  a.g = g; a.h = h; a.norm_dtype = norm_dtype; a.eps = (float)eps; a.act = act;
-  if (dtype == PYGHO_F32) return la_forward<float>(a, norm, (hipStream_t)stream);
-  return dtype == PYGHO_BF16 ? la_forward<bf16>(a, norm, (hipStream_t)stream) : la_forward<f16>(a, norm, (hipStream_t)stream);
+  hipStream_t st = (hipStream_t)stream;
+  if (la_streams(k, n, norm, dtype)) {
+    const LsArgs a = la_stream_args(x, x_ld, w, w_ld, bias, bias_dtype, g, h, norm_dtype, residual, residual_ld, y, m, k, n, eps, act, dtype);
+    return la_type(dtype, [&](auto ops) { return ops.stream_fwd(a, norm, st); });
+  }
+  if (!norm) return la_tile_act(x, x_ld, w, w_ld, bias, bias_dtype, residual, residual_ld, y, z, 0, m, k, n, act, dtype, st);
+  if (!z) { set_error("linear_act: this norm needs the pre-activation's buffer (pygho_linear_act_keeps)"); return PYGHO_ERR_INVALID; }
+  if (int rc = la_tile_act(x, x_ld, w, w_ld, bias, bias_dtype, nullptr, 0, nullptr, z, 1, m, k, n, kActNone, dtype, st)) return rc;
+  return ln_fwd_launch(y, z, n, g, h, norm_dtype, residual, residual_ld, m, n, (float)eps, act, dtype, PYGHO_F32, st);
 }
 
-extern "C" int pygho_linear_act_dz_slabs(int64_t m) { return m <= 0 ? 0 : (int)std::min<int64_t>((ceil_div(m, 64) + 7) / 8 * 8, kLaNormGrid); }
-
-extern "C" int pygho_linear_act_dz(void* dz, float* slabs, int64_t slab_stride, int* n_slabs, const void* x, int64_t x_ld, const void* w, int64_t w_ld,
-                                   const void* bias, int bias_dtype, int norm, const void* g, const void* h, int norm_dtype, double eps,
-                                   const void* gy, int64_t gy_ld, int64_t m_cap, const int32_t* m_dev, int64_t k, int64_t n, int act, int dtype,
-                                   void* stream) {
-  if (int rc = la_check("linear_act_dz", m_cap, k, n, act, dtype)) return rc;
-  if (norm && (n > kLaNormMax || !(eps >= 0.0))) { set_error("linear_act_dz: a norm over at most %d channels, eps >= 0", kLaNormMax); return PYGHO_ERR_UNSUPPORTED; }
-  if (!n_slabs || (norm && slab_stride < 2 * n)) { set_error("linear_act_dz: n_slabs, and 2 n floats per slab"); return PYGHO_ERR_INVALID; }
-  *n_slabs = 0;
-  if (m_cap == 0) return PYGHO_OK;
-  if (!dz || !x || !w || !gy || (norm && !slabs)) { set_error("null pointer"); return PYGHO_ERR_INVALID; }
-  const int es = dtype == PYGHO_F32 ? 4 : 2;
-  LaArgs a{};
-  a.a = la_operand(x, x_ld, dtype);
-  a.b = la_operand(w, w_ld, dtype);
-  a.m = m_cap; a.n = n; a.k = k; a.m_dev = m_dev;
-  a.out = dz; a.out_ld = n; a.out_vec = la_aligned(dz, n, es, 4 * es);
-  a.bias = bias; a.bias_dtype = bias_dtype;
-  a.res = gy; a.res_ld = gy_ld; a.res_vec = la_aligned(gy, gy_ld, es, 4 * es);
-  a.g = g; a.h = h; a.norm_dtype = norm_dtype; a.eps = (float)eps; a.act = act;
-  a.slabs = slabs; a.slab_stride = slab_stride;
-  if (dtype == PYGHO_F32) return la_dz<float>(a, norm, (hipStream_t)stream, norm ? n_slabs : nullptr);
-  return dtype == PYGHO_BF16 ? la_dz<bf16>(a, norm, (hipStream_t)stream, norm ? n_slabs : nullptr)
-                             : la_dz<f16>(a, norm, (hipStream_t)stream, norm ? n_slabs : nullptr);
+extern "C" size_t pygho_linear_act_bwd_workspace(int64_t m, int64_t k, int64_t n, int norm, int act, int dtype) {
+  if (m <= 0 || k <= 0 || n <= 0 || !ro_float(dtype)) return 0;
+  return (size_t)la_space(m, k, n, norm, act, dtype).total;
 }
 
-extern "C" int pygho_linear_dx(void* gx, const void* dz, int64_t dz_ld, const void* w, int64_t w_ld, int64_t m, int64_t k, int64_t n, int dtype,
-                               void* stream) {
-  if (int rc = la_check("linear_dx", m, k, n, 0, dtype)) return rc;
-  if (m == 0) return PYGHO_OK;
-  if (!gx || !dz || !w) { set_error("null pointer"); return PYGHO_ERR_INVALID; }
-  const int es = dtype == PYGHO_F32 ? 4 : 2;
-  LaArgs a{};
-  a.a = la_operand(dz, dz_ld, dtype);
-  a.b = la_operand(w, w_ld, dtype);                     // W (n, k): stored with the OUTPUT channel k of this product contiguous
-  a.m = m; a.n = k; a.k = n;
-  a.out = gx; a.out_ld = k; a.out_vec = la_aligned(gx, k, es, 4 * es);
-  if (dtype == PYGHO_F32) return la_dx<float>(a, (hipStream_t)stream);
-  return dtype == PYGHO_BF16 ? la_dx<bf16>(a, (hipStream_t)stream) : la_dx<f16>(a, (hipStream_t)stream);
-}
-
-// slabs of a weight gradient: enough workgroups for two per CU, at most one per chunk of rows
-extern "C" int pygho_linear_dw_slabs(int64_t m, int64_t k, int64_t n) {
-  if (m <= 0 || k <= 0 || n <= 0) return 0;
-  const int64_t tiles = (n > 64 && k > 64) ? ceil_div(n, 128) * ceil_div(k, 128) : ceil_div(n, 64) * ceil_div(k, k <= 16 ? 16 : 64);
-  return (int)std::min<int64_t>(ceil_div(m, kLaChunk), std::max<int64_t>(1, 512 / tiles));
-}
-
-extern "C" int pygho_linear_dw(float* slabs, int64_t slab_stride, const void* dz, int64_t dz_ld, const void* x, int64_t x_ld, int64_t m_cap,
-                               const int32_t* m_dev, int64_t k, int64_t n, int want_colsum, int dtype, void* stream) {
-  if (int rc = la_check("linear_dw", m_cap, k, n, 0, dtype)) return rc;
-  if (slab_stride < n * k + (want_colsum ? n : 0)) { set_error("linear_dw: slab_stride below n k (+ n)"); return PYGHO_ERR_INVALID; }
-  if (m_cap == 0) return PYGHO_OK;
-  if (!slabs || !dz || !x) { set_error("null pointer"); return PYGHO_ERR_INVALID; }
-  LaArgs a{};
-  a.a = la_operand(dz, dz_ld, dtype);
-  a.b = la_operand(x, x_ld, dtype);
-  a.m = n; a.n = k; a.k = m_cap; a.k_dev = m_dev;
-  a.slabs = slabs; a.slab_stride = slab_stride; a.splits = pygho_linear_dw_slabs(m_cap, k, n); a.want_sums = want_colsum;
-  if (dtype == PYGHO_F32) return la_dw<float>(a, (hipStream_t)stream);
-  return dtype == PYGHO_BF16 ? la_dw<bf16>(a, (hipStream_t)stream) : la_dw<f16>(a, (hipStream_t)stream);
+extern "C" int pygho_linear_act_bwd(void* gx, void* gw, int gw_dtype, void* gb, int gb_dtype, void* gg, int gg_dtype, void* gh, int gh_dtype,
+                                    const void* z, const void* x, int64_t x_ld, const void* w, int64_t w_ld, const void* bias, int bias_dtype,
+                                    int norm, const void* g, const void* h, int norm_dtype, double eps, const void* gy, int64_t gy_ld,
+                                    int64_t m_cap, const int32_t* m_dev, int64_t k, int64_t n, int act, int dtype, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  if (int rc = la_check("linear_act_bwd", m_cap, k, n, eps, act, dtype)) return rc;
+  if (int rc = la_param_check("linear_act_bwd", bias, bias_dtype, dtype)) return rc;
+  if (g || h) { if (int rc = la_param_check("linear_act_bwd", g ? g : h, norm_dtype, dtype)) return rc; }
+  if ((gw && !ro_float(gw_dtype)) || (gb && !ro_float(gb_dtype)) || (gg && !ro_float(gg_dtype)) || (gh && !ro_float(gh_dtype)) || (!norm && (gg || gh))) {
+    set_error("linear_act_bwd: gradients in f32 / bf16 / f16; gg and gh with a norm only");
+    return PYGHO_ERR_UNSUPPORTED;
+  }
+  if (int rc = la_stride_check("linear_act_bwd", x_ld, gy_ld, dtype)) return rc;
+  const LaSpace sp = la_space(m_cap, k, n, norm, act, dtype);
+  hipStream_t st = (hipStream_t)stream;
+  if (m_cap == 0) {                                           // no rows: every gradient of a parameter is zero
+    if (int rc = fold_launch(FoldOut{{gw, gb, gg, gh}, {gw ? n * k : 0, gb ? n : 0, gg ? n : 0, gh ? n : 0}, {gw_dtype, gb_dtype, gg_dtype, gh_dtype}}, nullptr, 0, 0, st)) return rc;
+    return PYGHO_OK;
+  }
+  if (!x || !w || !gy || !workspace) { set_error("null pointer"); return PYGHO_ERR_INVALID; }
+  if (workspace_bytes < (size_t)sp.total || (uintptr_t)workspace % 16 != 0) { set_error("linear_act_bwd: workspace too small or not 16-byte aligned"); return PYGHO_ERR_INVALID; }
+  if (pygho_linear_act_keeps(k, n, norm, act, dtype) != 0 && !z) { set_error("linear_act_bwd: the kept pre-activation is missing"); return PYGHO_ERR_INVALID; }
+  const int es = la_size(dtype);
+  char* base = reinterpret_cast<char*>(workspace);
+  const void* dz = gy;
+  int64_t dz_ld = gy_ld;
+  bool have_gx = gx == nullptr;
+  if (sp.own_dz) {
+    void* own = base;
+    float* slabs = reinterpret_cast<float*>(base + sp.dz + sp.z);
+    int64_t stride = la_pad4(sp.nsum * n);
+    int used = 0;
+    if (sp.stream) {
+      LsArgs a = la_stream_args(x, x_ld, w, w_ld, bias, bias_dtype, g, h, norm_dtype, gy, gy_ld, own, m_cap, k, n, eps, act, dtype);
+      a.m_dev = m_dev;
+      a.slabs = slabs; a.slab_stride = stride;
+      if (gx && la_type(dtype, [&](auto ops) { return ops.stream_dx_fits(k, n, norm); })) {
+        a.gx = gx;
+        a.vec = a.vec && la_aligned(gx, k, es, 4 * es);
+        have_gx = true;
+      }
+      if (int rc = la_type(dtype, [&](auto ops) { return ops.stream_bwd(a, norm, &used, st); })) return rc;
+    } else {
+      if (sp.z) {
+        LsArgs a = la_stream_args(x, x_ld, w, w_ld, bias, bias_dtype, nullptr, nullptr, 0, nullptr, 0, base + sp.dz, m_cap, k, n, 0.0, kActNone, dtype);
+        a.out_f32 = 1;
+        if (int rc = la_type(dtype, [&](auto ops) { return ops.stream_fwd(a, 0, st); })) return rc;
+        z = base + sp.dz;
+      }
+      if (int rc = ln_bwd_launch(own, slabs, &stride, &used, sp.nsum, z, n, gy, gy_ld, g, h, norm_dtype, m_cap, m_dev, n, (float)eps, act, dtype,
+                                 norm || sp.z ? PYGHO_F32 : dtype, st)) return rc;
+    }
+    dz = own;
+    dz_ld = n;
+    if (gb || gg || gh) {
+      const FoldOut o = norm ? FoldOut{{gg, gh, gb, nullptr}, {n, n, n, 0}, {gg_dtype, gh_dtype, gb_dtype, 0}}
+                             : FoldOut{{gb, nullptr, nullptr, nullptr}, {n, 0, 0, 0}, {gb_dtype, 0, 0, 0}};
+      if (int rc = fold_launch(o, slabs, used, stride, st)) return rc;
+    }
+  }
+  if (!have_gx) {
+    // dX = dz . W: a product over n with k output channels
+    if (la_streams(n, k, 0, dtype)) {
+      LsArgs a = la_stream_args(dz, dz_ld, w, w_ld, nullptr, 0, nullptr, nullptr, 0, nullptr, 0, gx, m_cap, n, k, 0.0, kActNone, dtype);
+      a.w_trans = 1;
+      if (int rc = la_type(dtype, [&](auto ops) { return ops.stream_fwd(a, 0, st); })) return rc;
+    } else {
+      LaArgs a{};
+      a.a = la_operand(dz, dz_ld, dtype);
+      a.b = la_operand(w, w_ld, dtype);
+      a.m = m_cap; a.n = k; a.k = n;
+      a.out = gx; a.out_vec = la_aligned(gx, k, es, 4 * es);
+      if (int rc = la_type(dtype, [&](auto ops) { return ops.tile_dx(a, st); })) return rc;
+    }
+  }
+  const bool db_here = gb && !sp.own_dz;                      // dz is gy itself: its column sums come with dW
+  if (gw || db_here) {
+    LaArgs a{};
+    a.a = la_operand(dz, dz_ld, dtype);
+    a.b = la_operand(x, x_ld, dtype);
+    a.m = n; a.n = k; a.k = m_cap; a.k_dev = m_dev;
+    a.slabs = reinterpret_cast<float*>(base + sp.dz + sp.z + sp.sums);
+    a.slab_stride = la_pad4(n * k + n);
+    a.splits = (int)la_dw_slabs(m_cap, k, n);
+    a.want_sums = db_here;
+    if (int rc = la_type(dtype, [&](auto ops) { return ops.tile_dw(a, st); })) return rc;
+    const FoldOut o{{gw, db_here ? gb : nullptr, nullptr, nullptr}, {n * k, db_here ? n : 0, 0, 0}, {gw_dtype, gb_dtype, 0, 0}};
+    if (int rc = fold_launch(o, a.slabs, a.splits, a.slab_stride, st)) return rc;
+  }
+  return PYGHO_OK;
 }

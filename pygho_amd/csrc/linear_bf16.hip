@@ -1,5 +1,5 @@
-// The linear operators over bf16 rows (linear_tile.h).
-#include "linear_tile.h"
+// The linear operators over bf16 rows.
+#include "linear_ops.h"
 
 namespace pygho {
 PYGHO_LINEAR_TYPE(bf16)

@@ -1,5 +1,5 @@
-// The linear operators over f32 rows (linear_tile.h).
-#include "linear_tile.h"
+// The linear operators over f32 rows.
+#include "linear_ops.h"
 
 namespace pygho {
 PYGHO_LINEAR_TYPE(float)

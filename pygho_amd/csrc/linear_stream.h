@@ -1,0 +1,529 @@
+// Streaming form of the linear operators: W stays in LDS, every wavefront walks its own blocks of rows without a barrier.
+// The tuple-wise maps have K and N of one or two hundred and 10^5 .. 10^6 rows: a row moves 0.5 .. 2 KB and needs 2 K N operations, which
+// the matrix cores do in less time than HBM takes for the row.  What has to go well is the stream:
+//   * W (N x K, padded rows) is read once per workgroup and serves all its rows; a workgroup lives until the rows are done;
+//   * a block is 16 rows of one wavefront.  Its x fragments (lane = row, 16 bytes of k) are global loads straight into registers, the next
+//     block's are in flight during this block's products and epilogue; wavefronts never wait for each other;
+//   * swapped MFMA (D[n][m]): a lane ends up with 4 consecutive channels of ONE row, a row's channels sit in 4 lanes: bias (the accumulator's
+//     start value), norm, activation, residual and the store happen in those registers;
+//   * backward: dz leaves the epilogue in exactly the lanes and order in which the product dz . W wants its operand (the order of n inside
+//     a reduction is free as long as W's copy has the same one), so dX follows in the same launch without moving a value;
+//   * channel sums (gg, gh, gb) are taken from the unrounded f32 values, over a block's 16 rows by lane exchanges (ls_row_sums).
+// Block b of the rows belongs to wavefront b % (all wavefronts), so sums depend on the true row count only (see layer_norm.hip).
+#pragma once
+#include "linear_tile.h"
+
+namespace pygho {
+
+enum { LS_ACT = 0, LS_NORM = 1, LS_DACT = 2, LS_DNORM = 3 };
+
+struct LsArgs {
+  const void* x; int64_t x_ld;
+  const void* w; int64_t w_ld; int w_vec; int w_trans;        // w_trans: w is stored [k][n] (the W of dz . W)
+  const void* bias; int bias_dtype; const void* g; const void* h; int norm_dtype;
+  const void* r; int64_t r_ld;                                // residual (forward) / output gradient (backward)
+  void* out; int out_f32;                                     // y / dz; out_f32 (LS_ACT): f32 values as they are
+  void* gx;                                                   // backward, nullable: dX (rows of k)
+  float* slabs; int64_t slab_stride;                          // backward: LS_DACT [gb], LS_DNORM [gg | gh | gb]
+  int64_t m; const int32_t* m_dev; int k; int n; float eps; int act;
+  int vec;                                                    // see VEC
+  int red_bytes;                                              // bytes reserved for W and, at the end, for the reduction
+};
+
+template <typename T> struct Raw4 { using type = uint2; };
+template <> struct Raw4<float> { using type = uint4; };
+
+// 16 bytes of a row from p (left elements remain): vectors where the operand's rows are aligned, element by element otherwise; zeros past the end
+template <typename T> __device__ __forceinline__ uint4 ls_load16(const T* row, int off, int end, int vec) {
+  constexpr int E = 16 / (int)sizeof(T);
+  uint4 v = make_uint4(0u, 0u, 0u, 0u);
+  if (vec) {                                            // (aligned rows of whole vectors, or rows that reach beyond `end`)
+    if (off + E <= end) return *reinterpret_cast<const uint4*>(row + off);
+  }
+  if (off >= end) return v;
+  const int left = end - off;
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (sizeof(T) == 4) {
+      w[j] = j < left ? reinterpret_cast<const uint32_t*>(row + off)[j] : 0u;
+    } else {
+      const uint32_t lo = 2 * j < left ? reinterpret_cast<const uint16_t*>(row + off)[2 * j] : 0u;
+      const uint32_t hi = 2 * j + 1 < left ? reinterpret_cast<const uint16_t*>(row + off)[2 * j + 1] : 0u;
+      w[j] = lo | (hi << 16);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <typename T> __device__ __forceinline__ typename Raw4<T>::type ls_load4(const T* row, int off, int end, int vec) {
+  typename Raw4<T>::type v{};
+  if (vec && off + 4 <= end) return *reinterpret_cast<const typename Raw4<T>::type*>(row + off);
+  if (off >= end) return v;
+  const int left = end - off;
+  if constexpr (sizeof(T) == 4) {
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(row + off);
+    v.x = p[0];
+    v.y = left > 1 ? p[1] : 0u;
+    v.z = left > 2 ? p[2] : 0u;
+    v.w = left > 3 ? p[3] : 0u;
+  } else {
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(row + off);
+    v.x = (uint32_t)p[0] | (left > 1 ? (uint32_t)p[1] << 16 : 0u);
+    v.y = (left > 2 ? (uint32_t)p[2] : 0u) | (left > 3 ? (uint32_t)p[3] << 16 : 0u);
+  }
+  return v;
+}
+template <typename T> __device__ __forceinline__ void ls_unpack4(const typename Raw4<T>::type& r, float (&v)[4]) {
+  if constexpr (sizeof(T) == 4) {
+    v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
+  } else {
+    float t[8];
+    Vec16<T>::unpack(make_uint4(r.x, r.y, 0u, 0u), t);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = t[i];
+  }
+}
+
+// Sums over the 16 rows of a block (lanes r16 of a group): V values per lane -> their totals dealt out over the lanes.  A step gives half of the values
+// to the partner lane and takes the partner's half of the others: V / 2 additions instead of V.  Partners i ^ 15, ^ 7, ^ 3, ^ 1 are single DPP
+// moves; `up[s]` says which half a lane keeps (bit 3 - s of its number).  Lane i ends up with values [i * V / 16, + V / 16); below 16 values the
+// steps that are left are plain sums.  Held per lane instead, the sums of 128 channels took 96 registers and one wavefront per SIMD less
+template <int V, int S> __device__ __forceinline__ void ls_row_sums(float (&v)[V], const bool (&up)[4]) {
+  constexpr int ctrl[4] = {0x140, 0x141, 0x1B, 0xB1};
+  if constexpr (V == 1) {
+    v[0] += ro_dpp<ctrl[S]>(v[0]);
+    if constexpr (S < 3) ls_row_sums<1, S + 1>(v, up);
+  } else {
+    float w[V / 2];
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) {
+      const float keep = up[S] ? v[j + V / 2] : v[j], send = up[S] ? v[j] : v[j + V / 2];
+      w[j] = keep + ro_dpp<ctrl[S]>(send);
+    }
+    if constexpr (S < 3) ls_row_sums<V / 2, S + 1>(w, up);
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) v[j] = w[j];
+  }
+}
+
+// position of reduction index n in the transposed copy of W: the order in which a lane's accumulators hold it.  16-bit: a step is 32 n, lane
+// group q holds 4 q .. 4 q + 3 of its first and of its second 16; f32: a step is 16 n, lane group q holds 4 q .. 4 q + 3
+template <typename T> __device__ __forceinline__ int ls_perm(int n) {
+  if constexpr (sizeof(T) == 4) return n;
+  return (n & ~31) | (((n >> 2) & 3) << 3) | (((n >> 4) & 1) << 2) | (n & 3);
+}
+
+constexpr int kLsThreads = 512;
+
+// geometry that host and device share
+template <typename T, int NB> struct LsGeom {
+  static constexpr int ES = sizeof(T), NP = NB * 16;
+  static constexpr int NS = (NP * ES + 63) / 64;               // 64-byte steps over n (dX)
+  static constexpr int PITCH_T = NS * 64 + 16;                 // a row of the transposed copy
+  __host__ __device__ static int steps(int k) { return (k * ES + 63) / 64; }
+  __host__ __device__ static int pitch_w(int k) { return steps(k) * 64 + 16; }
+  __host__ __device__ static int rows_t(int k) { return (k + 15) / 16 * 16; }
+  __host__ __device__ static int w_bytes(int k) { return NP * pitch_w(k); }
+  __host__ __device__ static int t_bytes(int k) { return rows_t(k) * PITCH_T; }
+  static constexpr int param_bytes = 4 * NP * 4;
+};
+
+// VEC: k is a whole number of 64-byte steps, n of 16 channels, and every row of x, r, out and gx allows 16-byte (x) / 4-element accesses.  A block's
+// rows then are one uniform base address, one 32-bit offset per lane and constants -- 64-bit addresses per access, or masks per element, take
+// more registers than the sums do.  Otherwise element by element
+template <typename T, int NB, int EPI, bool DX, bool VEC>
+__global__ __launch_bounds__(kLsThreads) void linear_stream_kernel(LsArgs a) {
+  using G = LsGeom<T, NB>;
+  constexpr bool P = Precise<T>::value, BWD = EPI == LS_DACT || EPI == LS_DNORM, NORM = EPI == LS_NORM || EPI == LS_DNORM;
+  constexpr int ES = G::ES, E = 16 / ES, NP = G::NP, KC = 4;
+  constexpr int NSUM = EPI == LS_DNORM ? 3 : EPI == LS_DACT ? 1 : 0;      // sums per channel
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int K = a.k, N = a.n, KS = G::steps(K), pitch = G::pitch_w(K);
+  char* lds_w = smem;
+  float* lds_bias = reinterpret_cast<float*>(smem + a.red_bytes);
+  float* lds_g = lds_bias + NP;
+  float* lds_h = lds_g + NP;
+  float* lds_on = lds_h + NP;                                  // 1 for a channel of the row, 0 for padding (comparisons would hold 32 masks)
+  char* lds_t = smem + a.red_bytes + G::param_bytes;
+  const int lane = threadIdx.x & 63, wave = PYGHO_WAVE_INDEX(threadIdx.x >> 6), r16 = lane & 15, q = lane >> 4;
+  const T* wp = reinterpret_cast<const T*>(a.w);
+
+  // ---- W -> LDS (padding: zeros) ----------------------------------------------------------------------------------------------------
+  if (!a.w_trans) {
+    const int cpr = KS * 4;                                    // 16-byte chunks per row
+    for (int c = threadIdx.x; c < NP * cpr; c += blockDim.x) {
+      const int n = c / cpr, kc = c - n * cpr;
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (n < N) v = ls_load16<T>(wp + (int64_t)n * a.w_ld, kc * E, K, a.w_vec);
+      *reinterpret_cast<uint4*>(lds_w + n * pitch + kc * 16) = v;
+    }
+  } else {
+    constexpr int CN = NP / E;
+    const int kp = KS * 64 / ES;
+    for (int c = threadIdx.x; c < kp * CN; c += blockDim.x) {
+      const int k = c / CN, nc = c - k * CN;
+      union { uint4 u; uint16_t h[8]; uint32_t f[4]; } v;
+      v.u = make_uint4(0u, 0u, 0u, 0u);
+      if (k < K) v.u = ls_load16<T>(wp + (int64_t)k * a.w_ld, nc * E, N, a.w_vec);
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        if constexpr (ES == 2) *reinterpret_cast<uint16_t*>(lds_w + (nc * E + j) * pitch + k * 2) = v.h[j];
+        else *reinterpret_cast<uint32_t*>(lds_w + (nc * E + j) * pitch + k * 4) = v.f[j];
+      }
+    }
+  }
+  if constexpr (DX) {                                          // the copy with n contiguous: rows k, columns ls_perm(n)
+    const int kr = G::rows_t(K), ck = (kr + E - 1) / E, np = G::NS * 64 / ES;
+    for (int c = threadIdx.x; c < np * ck; c += blockDim.x) {
+      const int n = c / ck, kc = c - n * ck, pn = ls_perm<T>(n);
+      union { uint4 u; uint16_t h[8]; uint32_t f[4]; } v;
+      v.u = make_uint4(0u, 0u, 0u, 0u);
+      if (n < N) v.u = ls_load16<T>(wp + (int64_t)n * a.w_ld, kc * E, K, a.w_vec);
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const int k = kc * E + j;
+        if (k >= kr) break;
+        if constexpr (ES == 2) *reinterpret_cast<uint16_t*>(lds_t + k * G::PITCH_T + pn * 2) = v.h[j];
+        else *reinterpret_cast<uint32_t*>(lds_t + k * G::PITCH_T + pn * 4) = v.f[j];
+      }
+    }
+  }
+  for (int n = threadIdx.x; n < NP; n += blockDim.x) {
+    lds_bias[n] = n < N ? ro_param(a.bias, a.bias_dtype, n, 0.f) : 0.f;
+    lds_g[n] = n < N ? ro_param(a.g, a.norm_dtype, n, 1.f) : 0.f;
+    lds_h[n] = n < N ? ro_param(a.h, a.norm_dtype, n, 0.f) : 0.f;
+    lds_on[n] = n < N ? 1.f : 0.f;
+  }
+  __syncthreads();
+
+  int64_t m_rows = a.m;
+  if (BWD && a.m_dev) m_rows = *a.m_dev;
+  const int waves = blockDim.x >> 6;
+  const int64_t n_blocks = (m_rows + 15) / 16, stride = (int64_t)gridDim.x * waves;
+  const int nk = (KS + KC - 1) / KC;
+  const bool n_full = N == NP;
+  const float inv_n = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, 1.f / (float)N)));
+
+  constexpr int VS = NB * 4 / 16 > 0 ? NB * 4 / 16 : 1;        // channels of a lane's 4 NB whose sums it keeps (ls_row_sums)
+  float sums[NSUM ? NSUM : 1][VS];
+#pragma unroll
+  for (int s = 0; s < (NSUM ? NSUM : 1); ++s)
+#pragma unroll
+    for (int i = 0; i < VS; ++i) sums[s][i] = 0.f;
+  const bool up[4] = {(lane & 8) != 0, (lane & 4) != 0, (lane & 2) != 0, (lane & 1) != 0};
+  auto add_rows = [&](int s, float (&t)[NB * 4]) {
+    ls_row_sums<NB * 4, 0>(t, up);
+#pragma unroll
+    for (int i = 0; i < VS; ++i) sums[s][i] += t[i];
+  };
+
+  // the block's rows from b0 on: this lane's row (a row past the end repeats the last one and is never stored), as bytes from the block's first row
+  auto lane_row = [&](int64_t b) { return min(r16, (int)min((int64_t)15, m_rows - 1 - b * 16)); };
+  uint4 xc[KC], xn[KC];
+  auto load_x = [&](int64_t b, int kc, uint4 (&dst)[KC]) {
+    const char* base = reinterpret_cast<const char*>(a.x) + b * 16 * a.x_ld * ES + kc * (KC * 64);
+    const uint32_t off = (uint32_t)lane_row(b) * (uint32_t)(a.x_ld * ES) + (VEC ? q * 16 : 0);
+#pragma unroll
+    for (int s = 0; s < KC; ++s) {
+      if constexpr (VEC) {
+        if (kc * KC + s < KS) dst[s] = *reinterpret_cast<const uint4*>(base + off + s * 64);
+      } else {
+        dst[s] = ls_load16<T>(reinterpret_cast<const T*>(base + off), s * (64 / ES) + q * E, K - kc * (KC * 64 / ES), 0);
+      }
+    }
+  };
+  int64_t blk = (int64_t)blockIdx.x * waves + wave;
+  if (blk < n_blocks) load_x(blk, 0, xc);
+  for (; blk < n_blocks; blk += stride) {
+    // the parameters are read from LDS block after block: hoisted out of the loop they would take up to 96 registers
+    asm volatile("" ::: "memory");
+    const bool row_ok = r16 <= (int)min((int64_t)15, m_rows - 1 - blk * 16);
+    // the residual's / the output gradient's 4 channels per lane and 16: in flight during the products
+    typename Raw4<T>::type rv[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) rv[nb] = typename Raw4<T>::type{};
+    if (a.r) {
+      const char* base = reinterpret_cast<const char*>(a.r) + blk * 16 * a.r_ld * ES;
+      const uint32_t off = (uint32_t)lane_row(blk) * (uint32_t)(a.r_ld * ES) + (VEC ? q * 4 * ES : 0);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        if constexpr (VEC) {
+          if (n_full || nb * 16 < N) rv[nb] = *reinterpret_cast<const typename Raw4<T>::type*>(base + off + nb * 16 * ES);
+        } else {
+          rv[nb] = ls_load4<T>(reinterpret_cast<const T*>(base + off), nb * 16 + q * 4, N, 0);
+        }
+      }
+    }
+    la_f32x4_t acc[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) acc[nb] = *reinterpret_cast<const la_f32x4_t*>(lds_bias + nb * 16 + q * 4);
+    for (int kc = 0; kc < nk; ++kc) {
+      if (kc + 1 < nk) load_x(blk, kc + 1, xn);
+      else load_x(min(blk + stride, n_blocks - 1), 0, xn);
+#pragma unroll
+      for (int s = 0; s < KC; ++s) {
+        if (kc * KC + s < KS) {
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            const uint4 fa = *reinterpret_cast<const uint4*>(lds_w + (nb * 16 + r16) * pitch + (kc * KC + s) * 64 + q * 16);
+            acc[nb] = la_mfma<T>(fa, xc[s], acc[nb]);
+          }
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < KC; ++s) xc[s] = xn[s];
+    }
+    {
+      float v[NB][4], rstd = 0.f;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[nb][e] = acc[nb][e];
+      if constexpr (NORM) {                                    // v becomes xh; channels beyond N are zero throughout
+        float s = 0.f, ss = 0.f;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s += v[nb][e];
+        const float mean = la_q_sum(s) * inv_n;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[nb][e] -= mean;
+        if (!n_full) {
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[nb][e] *= lds_on[nb * 16 + q * 4 + e];
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ss = fmaf(v[nb][e], v[nb][e], ss);
+        rstd = 1.f / sqrtf(la_q_sum(ss) * inv_n + a.eps);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[nb][e] *= rstd;
+      }
+      // where this lane's channels of its row go: byte offset from the block's first row
+      auto store_rows = [&](auto* rows, float (&val)[NB][4], int64_t width) {
+        using O = std::remove_reference_t<decltype(*rows)>;
+        char* base = reinterpret_cast<char*>(rows) + blk * 16 * width * (int64_t)sizeof(O);
+        const uint32_t off = (uint32_t)r16 * (uint32_t)(width * sizeof(O)) + q * 4 * sizeof(O);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+          if ((VEC ? nb * 16 : nb * 16 + q * 4) < N)
+            la_store4<O>(reinterpret_cast<O*>(base + off + nb * 16 * sizeof(O)), VEC ? 4 : N - nb * 16 - q * 4, VEC, val[nb]);
+      };
+      // (channel block by channel block: whole-row arrays of intermediates do not fit beside the sums and the next block's x)
+      if constexpr (!BWD) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          const int n = nb * 16 + q * 4;
+          if constexpr (NORM) {
+            const float4 g4 = *reinterpret_cast<const float4*>(lds_g + n), h4 = *reinterpret_cast<const float4*>(lds_h + n);
+            v[nb][0] = fmaf(v[nb][0], g4.x, h4.x); v[nb][1] = fmaf(v[nb][1], g4.y, h4.y);
+            v[nb][2] = fmaf(v[nb][2], g4.z, h4.z); v[nb][3] = fmaf(v[nb][3], g4.w, h4.w);
+          }
+          ro_act<P, 4>(v[nb], a.act);
+          float r4[4];
+          ls_unpack4<T>(rv[nb], r4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[nb][e] += r4[e];
+        }
+        if (row_ok) {
+          if (EPI == LS_ACT && a.out_f32) store_rows(reinterpret_cast<float*>(a.out), v, N);
+          else store_rows(reinterpret_cast<T*>(a.out), v, N);
+        }
+      } else {
+        float d[NB][4], k1 = 0.f, k2 = 0.f;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          const int n = nb * 16 + q * 4;
+          ls_unpack4<T>(rv[nb], d[nb]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) d[nb][e] = row_ok ? d[nb][e] : 0.f;      // a repeated row adds nothing to the sums
+          if constexpr (NORM) {
+            const float4 g4 = *reinterpret_cast<const float4*>(lds_g + n);
+            const float gv[4] = {g4.x, g4.y, g4.z, g4.w};
+            if (a.act != kActNone) {
+              const float4 h4 = *reinterpret_cast<const float4*>(lds_h + n);
+              const float z[4] = {fmaf(v[nb][0], g4.x, h4.x), fmaf(v[nb][1], g4.y, h4.y), fmaf(v[nb][2], g4.z, h4.z), fmaf(v[nb][3], g4.w, h4.w)};
+              ro_act_slope<P, 4>(d[nb], z, a.act);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float ev = d[nb][e] * gv[e];
+              k1 += ev;
+              k2 = fmaf(ev, v[nb][e], k2);
+            }
+          } else {
+            if (a.act != kActNone) ro_act_slope<P, 4>(d[nb], v[nb], a.act);
+          }
+        }
+        if constexpr (NORM) {
+          k1 = la_q_sum(k1) * inv_n;
+          k2 = la_q_sum(k2) * inv_n;
+          // (a repeated row's gy is zero: it adds nothing)
+          float t[NB * 4];
+#pragma unroll
+          for (int i = 0; i < NB * 4; ++i) t[i] = d[i / 4][i % 4] * v[i / 4][i % 4];
+          add_rows(0, t);
+#pragma unroll
+          for (int i = 0; i < NB * 4; ++i) t[i] = d[i / 4][i % 4];
+          add_rows(NSUM > 1 ? 1 : 0, t);
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          const int n = nb * 16 + q * 4;
+          if constexpr (NORM) {
+            const float4 g4 = *reinterpret_cast<const float4*>(lds_g + n);
+            const float gv[4] = {g4.x, g4.y, g4.z, g4.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[nb][e] = rstd * fmaf(-v[nb][e], k2, fmaf(d[nb][e], gv[e], -k1));
+            if (!n_full) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) d[nb][e] *= lds_on[n + e];
+            }
+          }
+        }
+        {                                                      // (gy = 0 gives dz = 0 through the norm too)
+          float t[NB * 4];
+#pragma unroll
+          for (int i = 0; i < NB * 4; ++i) t[i] = d[i / 4][i % 4];
+          add_rows(NSUM ? NSUM - 1 : 0, t);
+        }
+        if (row_ok) store_rows(reinterpret_cast<T*>(a.out), d, N);
+        if constexpr (DX) {
+          // dz as the operand of dz . W: step s of n = this lane's registers 2 s, 2 s + 1 (16-bit, rounded once) or s (f32)
+          uint4 f[G::NS];
+#pragma unroll
+          for (int s = 0; s < G::NS; ++s) {
+            if constexpr (ES == 4) {
+              f[s] = make_uint4(__float_as_uint(d[s][0]), __float_as_uint(d[s][1]), __float_as_uint(d[s][2]), __float_as_uint(d[s][3]));
+            } else {
+              float t[8];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) { t[e] = d[2 * s][e]; t[4 + e] = 2 * s + 1 < NB ? d[2 * s + 1 < NB ? 2 * s + 1 : 0][e] : 0.f; }
+              f[s] = Vec16<T>::pack(t);
+            }
+          }
+          char* base = reinterpret_cast<char*>(a.gx) + blk * 16 * K * ES;
+          const uint32_t off = (uint32_t)r16 * (uint32_t)(K * ES) + q * 4 * ES;
+          const int kb_end = (K + 15) / 16;
+          for (int kg = 0; kg < kb_end; kg += 4) {
+            la_f32x4_t o[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) o[t] = la_f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < G::NS; ++s)
+#pragma unroll
+              for (int t = 0; t < 4; ++t) {
+                const int kb = min(kg + t, kb_end - 1);        // (a block past the end is formed again and not stored)
+                const uint4 fa = *reinterpret_cast<const uint4*>(lds_t + (kb * 16 + r16) * G::PITCH_T + s * 64 + q * 16);
+                o[t] = la_mfma<T>(fa, f[s], o[t]);
+              }
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              const int k = (kg + t) * 16 + q * 4;
+              const float o4[4] = {o[t][0], o[t][1], o[t][2], o[t][3]};
+              if (row_ok && k < K) la_store4<T>(reinterpret_cast<T*>(base + (kg + t) * 16 * ES + off), VEC ? 4 : K - k, VEC, o4);
+            }
+          }
+        }
+      }
+    }
+  }
+  if constexpr (NSUM > 0) {
+    // lanes of a channel group -> wavefronts (in wave order) -> this workgroup's slab.  The buffer is W's place
+    float* red = reinterpret_cast<float*>(smem);
+    __syncthreads();
+    constexpr int SAME = NB >= 4 ? 1 : 4 / NB;                 // (fewer than 16 values: so many lanes hold the same one)
+    if (r16 % SAME == 0) {
+#pragma unroll
+      for (int i = 0; i < VS; ++i) {
+        const int idx = r16 / SAME * VS + i;
+#pragma unroll
+        for (int t = 0; t < NSUM; ++t) red[(wave * NSUM + t) * NP + (idx >> 2) * 16 + q * 4 + (idx & 3)] = sums[t][i];
+      }
+    }
+    __syncthreads();
+    float* slab = a.slabs + (int64_t)blockIdx.x * a.slab_stride;
+    for (int c = threadIdx.x; c < NSUM * NP; c += blockDim.x) {
+      const int s = c / NP, n = c - s * NP;
+      if (n >= N) continue;
+      float t = 0.f;
+      for (int w = 0; w < waves; ++w) t += red[(w * NSUM + s) * NP + n];
+      slab[(int64_t)s * N + n] = t;
+    }
+  }
+}
+
+// ---- launches ---------------------------------------------------------------------------------------------------------------------------
+constexpr int kLsLds = 158 * 1024;                             // a CU has 160 KB
+constexpr int ls_nb(int64_t n) { return n <= 16 ? 1 : n <= 32 ? 2 : n <= 64 ? 4 : n <= 128 ? 8 : n <= 256 ? 16 : 0; }
+
+template <typename T, int NB> static int ls_lds(int k, int sums, bool dx) {
+  using G = LsGeom<T, NB>;
+  const int red = std::max(G::w_bytes(k), (kLsThreads / kWave) * sums * G::NP * 4);
+  return red + G::param_bytes + (dx ? G::t_bytes(k) : 0);
+}
+// bytes of LDS a launch over (k, n) needs (beyond kLsLds, or n beyond 256: the tiled product takes over)
+template <typename T> static int ls_lds_any(int64_t k, int64_t n, int sums, bool dx) {
+  if (k > 4096) return INT32_MAX;
+  switch (ls_nb(n)) {
+    case 1: return ls_lds<T, 1>((int)k, sums, dx);
+    case 2: return ls_lds<T, 2>((int)k, sums, dx);
+    case 4: return ls_lds<T, 4>((int)k, sums, dx);
+    case 8: return ls_lds<T, 8>((int)k, sums, dx);
+    case 16: return ls_lds<T, 16>((int)k, sums, dx);
+  }
+  return INT32_MAX;
+}
+
+// channels of a streaming backward pass: beyond 128, xh, dz and the temporaries of the three sums do not fit a lane's 256 registers
+constexpr int ls_bwd_max(int norm) { return norm ? 128 : 256; }
+constexpr int kLsGrid = 512;                                   // workgroups of a launch: two per CU where LDS and registers allow
+
+template <typename T, int NB, int EPI, bool DX, bool VEC> static int ls_go(LsArgs a, int* n_slabs, hipStream_t st) {
+  constexpr int NSUM = EPI == LS_DNORM ? 3 : EPI == LS_DACT ? 1 : 0;
+  const int lds = ls_lds<T, NB>(a.k, NSUM, DX);
+  a.red_bytes = lds - LsGeom<T, NB>::param_bytes - (DX ? LsGeom<T, NB>::t_bytes(a.k) : 0);
+  static bool attr_set_dev[64] = {};
+  bool& attr_set = per_device_flag(attr_set_dev);
+  if (!attr_set) {
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&linear_stream_kernel<T, NB, EPI, DX, VEC>), hipFuncAttributeMaxDynamicSharedMemorySize, kLsLds);
+    if (e != hipSuccess) { set_error("linear_stream: cannot reserve %d B of LDS: %s", kLsLds, hipGetErrorString(e)); return PYGHO_ERR_LAUNCH; }
+    attr_set = true;
+  }
+  // few rows: workgroups of 4 wavefronts, so that more CUs take part (a backward launch keeps 8: its sums must not depend on the row count's
+  // upper bound)
+  const int64_t blocks = ceil_div(a.m, 16);
+  const int threads = NSUM == 0 && blocks < 256 * 8 ? 256 : kLsThreads;
+  const int grid = (int)std::min<int64_t>(ceil_div(blocks, threads / kWave), lds <= 80 * 1024 ? kLsGrid : kLsGrid / 2);
+  if (n_slabs) *n_slabs = grid;
+  hipLaunchKernelGGL((linear_stream_kernel<T, NB, EPI, DX, VEC>), dim3(grid), dim3(threads), lds, st, a);
+  return check_launch("linear_stream");
+}
+
+// One 16-row block per wavefront and turn: the registers go to the epilogue, the sums and the prefetch, and reading W's fragments costs 16 of
+// the ~85 cycles that HBM takes per row at K = N = 128, 64 of 114 at 256
+template <typename T, int EPI, bool DX, bool VEC> static int ls_pick_vec(const LsArgs& a, int* n_slabs, hipStream_t st) {
+  switch (ls_nb(a.n)) {
+    case 1: return ls_go<T, 1, EPI, DX, VEC>(a, n_slabs, st);
+    case 2: return ls_go<T, 2, EPI, DX, VEC>(a, n_slabs, st);
+    case 4: return ls_go<T, 4, EPI, DX, VEC>(a, n_slabs, st);
+    case 8: return ls_go<T, 8, EPI, DX, VEC>(a, n_slabs, st);
+    case 16:
+      if constexpr (EPI != LS_DNORM) return ls_go<T, 16, EPI, DX, VEC>(a, n_slabs, st);
+      break;                                                   // ls_bwd_max
+  }
+  set_error("linear_stream: %d channels", a.n);
+  return PYGHO_ERR_UNSUPPORTED;
+}
+template <typename T, int EPI, bool DX> static int ls_pick(const LsArgs& a, int* n_slabs, hipStream_t st) {
+  return a.vec ? ls_pick_vec<T, EPI, DX, true>(a, n_slabs, st) : ls_pick_vec<T, EPI, DX, false>(a, n_slabs, st);
+}
+
+}  // namespace pygho

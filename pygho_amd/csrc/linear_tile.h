@@ -1,15 +1,9 @@
-// Linear maps of the MLPs with what surrounds them in one launch (reference honn/utils.py:126-138: Linear -> norm -> act; the residual
-// connection of example/zinc.py:287-290), for any width, row stride, alignment, f32 / bf16 / f16:
-//   forward         z = x W^T + b,  y = act(z) + r            or, with a layer norm over the N output channels in between,
-//                   y = act(xh g + h) + r,  xh = (z - mean_n z) / sqrt(var_n z + eps)
-//   gradient of z   z formed again from x (a tile's product costs less than writing z in the forward and reading it back),
-//                   dz = gy act'(z)     or through the norm: du = gy act'(xh g + h), e = du g, dz = rstd (e - mean e - xh mean(e xh))
-//   dX = dz W,      dW = dz^T x  (+ db = the column sums of dz)
-// One tiled product serves all of them.  Output element (m, n) = sum_k P(m, k) Q(n, k); an operand is stored with its k contiguous ("rows": x
-// and W of the forward, dz of dX) or with its m / n contiguous ("columns": W of dX, dz and x of dW).  A step of the k loop moves 128
-// bytes of k per row (64 16-bit or 32 f32 values) global -> registers -> LDS, one step ahead of the matrix instructions.  The MFMA runs in
-// the swapped form D[n][m]: a lane holds one row m and 4 consecutive n, so a row's channels sit in the 4 lanes {m, m + 16, m + 32, m + 48}
-// of ONE wavefront when the tile spans all N: the norm is two lane exchanges per sum, and the epilogue never leaves the registers.
+// Tiled product behind the linear operators where W does not fit a CU's LDS (linear_stream.h is the other form), and for the weight
+// gradient, whose long dimension is the reduction.  Any width, row stride, alignment, f32 / bf16 / f16.
+// Output element (m, n) = sum_k P(m, k) Q(n, k); an operand is stored with its k contiguous ("rows": x and W of the forward, dz of dX) or
+// with its m / n contiguous ("columns": W of dX, dz and x of dW).  A step of the k loop moves 128 bytes of k per row (64 16-bit or 32 f32
+// values) global -> registers -> LDS, one step ahead of the matrix instructions.  The MFMA runs in the swapped form D[n][m]: a lane holds one
+// row m and 4 consecutive n, which it stores as one vector.
 // Column operands stay in their storage order in LDS; 16-bit fragments are read back transposed by the LDS itself (ds_read_b64_tr_b16),
 // f32 ones element by element (conflict-free, and an f32 MFMA takes 32 cycles).
 // f32 products run on v_mfma_f32_16x16x4f32: true f32, no reduced-precision path.
@@ -24,8 +18,8 @@ typedef __attribute__((ext_vector_type(4))) float la_f32x4_t;
 typedef __attribute__((ext_vector_type(4))) short la_s4_t;
 
 enum { LA_ROWS = 0, LA_COLS = 1 };
-// epilogues: activation (+ residual); norm + activation (+ residual); gradient of z without / with the norm; f32 slab of a split product
-enum { LA_ACT = 0, LA_NORM = 1, LA_DACT = 2, LA_DNORM = 3, LA_SLAB = 4 };
+// epilogues: bias, activation, residual, one store (the pre-activation beside it if asked); f32 slab of a split product
+enum { LA_ACT = 0, LA_SLAB = 4 };
 
 struct LaOperand { const void* p; int64_t ld; int vec; };      // vec: rows on 16-byte boundaries (16-byte loads where they fit)
 
@@ -33,14 +27,13 @@ struct LaArgs {
   LaOperand a, b;                     // P (m, k), Q (n, k)
   int64_t m; int64_t n; int64_t k;    // k: of the whole product; LA_SLAB: an upper bound of it (k_dev: the true one)
   const int32_t* k_dev;
-  void* out; int64_t out_ld; int out_vec; int out_f32;  // out_f32: LA_ACT stores the f32 values as they are
+  void* out; int out_vec;             // nullable: only z
+  void* z; int z_f32; int z_vec;      // nullable: the pre-activation, in the storage type or in f32
   const void* bias; int bias_dtype;
-  const void* res; int64_t res_ld; int res_vec;       // forward: the residual; LA_DACT / LA_DNORM: the output gradient
-  const void* g; const void* h; int norm_dtype;
-  float eps; int act;
-  float* slabs; int64_t slab_stride; int splits;      // LA_SLAB: slab s = [m * n product | m column sums (want_sums)]; LA_DNORM: [gg | gh]
+  const void* res; int64_t res_ld; int res_vec;
+  int act;
+  float* slabs; int64_t slab_stride; int splits;      // LA_SLAB: slab s = [m * n product | m column sums (want_sums)]
   int want_sums;
-  const int32_t* m_dev;                               // LA_DNORM / LA_DACT: true row count
 };
 
 // one step of k (64 bytes per row): bf16 / f16 one 16x16x32 MFMA, f32 four 16x16x4 (element j of every lane's 4 is k = 4 q + j on both sides)
@@ -173,14 +166,13 @@ __global__ __launch_bounds__(kBlock) void linear_tile_kernel(LaArgs g) {
   constexpr int KE = TA::KE, TM = BM / WM, TN = BN / WN, NM = TM / 16, NN = TN / 16;
   constexpr bool P = Precise<T>::value;
   static_assert(WM * WN * kWave == kBlock && TM % 16 == 0 && TN % 16 == 0, "tile");
-  static_assert((EPI != LA_NORM && EPI != LA_DNORM) || WN == 1, "a row's channels stay in one wavefront");
   __shared__ __attribute__((aligned(16))) char lds_a[TA::BYTES];
   __shared__ __attribute__((aligned(16))) char lds_b[TB::BYTES];
   const int lane = threadIdx.x & 63, wave = PYGHO_WAVE_INDEX(threadIdx.x >> 6);
   const int r16 = lane & 15, q = lane >> 4;
   const int wm = (wave / WN) * TM, wn = (wave % WN) * TN;
-  int64_t m_rows = g.m, k_end = g.k;
-  if constexpr (EPI == LA_DACT || EPI == LA_DNORM) { if (g.m_dev) m_rows = *g.m_dev; }
+  const int64_t m_rows = g.m;
+  int64_t k_end = g.k;
   if constexpr (EPI == LA_SLAB) { if (g.k_dev) k_end = *g.k_dev; }
   const int64_t tiles_n = (g.n + BN - 1) / BN, tiles_m = (m_rows + BM - 1) / BM;
   const int splits = EPI == LA_SLAB ? g.splits : 1;
@@ -188,13 +180,6 @@ __global__ __launch_bounds__(kBlock) void linear_tile_kernel(LaArgs g) {
   // consecutive workgroups go to the 8 XCDs in turn: with several column tiles, an XCD takes a contiguous range of tiles (column tile
   // innermost), so that the row tile they share is read from HBM once and from that XCD's L2 after that
   const int64_t per_xcd = (tiles + 7) / 8;
-  float sg[EPI == LA_DNORM ? NN : 1][4], sh[EPI == LA_DNORM ? NN : 1][4];
-  if constexpr (EPI == LA_DNORM) {
-#pragma unroll
-    for (int nb = 0; nb < NN; ++nb)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { sg[nb][i] = 0.f; sh[nb][i] = 0.f; }
-  }
 
   for (int64_t slot = blockIdx.x; slot < per_xcd * 8; slot += gridDim.x) {
     const int64_t t = tiles_n * splits > 1 ? (slot & 7) * per_xcd + (slot >> 3) : slot;
@@ -279,142 +264,34 @@ __global__ __launch_bounds__(kBlock) void linear_tile_kernel(LaArgs g) {
       T* out = reinterpret_cast<T*>(g.out);
 #pragma unroll
       for (int j = 0; j < NN; ++j) {
-        float bv[4];
+        const int64_t n = n0 + wn + j * 16 + q * 4;
+        const int left = (int)min((int64_t)4, g.n - n);
+        if (left <= 0) continue;
+        float b4[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int64_t n = n0 + wn + j * 16 + q * 4 + e;
-          bv[e] = n < g.n ? ro_param(g.bias, g.bias_dtype, n, 0.f) : 0.f;
-        }
+        for (int e = 0; e < 4; ++e) b4[e] = e < left ? ro_param(g.bias, g.bias_dtype, n + e, 0.f) : 0.f;
 #pragma unroll
-        for (int i = 0; i < NM; ++i)
+        for (int i = 0; i < NM; ++i) {
+          const int64_t m = m0 + wm + i * 16 + r16;
+          if (m >= m_rows) continue;
+          float u[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][j][e] += bv[e];
-      }
-#pragma unroll
-      for (int i = 0; i < NM; ++i) {
-        const int64_t m = m0 + wm + i * 16 + r16;
-        const bool row_ok = m < m_rows;
-        float rstd = 0.f;
-        if constexpr (EPI == LA_NORM || EPI == LA_DNORM) {
-          // statistics of the row from its registers: mean, then the centred squares; acc becomes xh (absent channels: 0)
-          const float inv_n = 1.f / (float)g.n;
-          float s = 0.f, v = 0.f;
-#pragma unroll
-          for (int j = 0; j < NN; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s += acc[i][j][e];
-          const float mean = la_q_sum(s) * inv_n;
-#pragma unroll
-          for (int j = 0; j < NN; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float d = wn + j * 16 + q * 4 + e < g.n ? acc[i][j][e] - mean : 0.f;
-              acc[i][j][e] = d;
-              v = fmaf(d, d, v);
-            }
-          rstd = 1.f / sqrtf(la_q_sum(v) * inv_n + g.eps);
-#pragma unroll
-          for (int j = 0; j < NN; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i][j][e] *= rstd;
-        }
-        if constexpr (EPI == LA_ACT || EPI == LA_NORM) {
-#pragma unroll
-          for (int j = 0; j < NN; ++j) {
-            const int64_t n = n0 + wn + j * 16 + q * 4;
-            const int left = (int)min((int64_t)4, g.n - n);
-            float u[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-            if constexpr (EPI == LA_NORM) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                u[e] = e < left ? fmaf(u[e], ro_param(g.g, g.norm_dtype, n + e, 1.f), ro_param(g.h, g.norm_dtype, n + e, 0.f)) : 0.f;
-            }
-            ro_act<P, 4>(u, g.act);
-            if (row_ok && left > 0) {
-              if (res) {
-                float r[4];
-                la_load4<T>(res + m * g.res_ld + n, left, g.res_vec, r);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) u[e] += r[e];
-              }
-              if (EPI == LA_ACT && g.out_f32) la_store4<float>(reinterpret_cast<float*>(g.out) + m * g.out_ld + n, left, g.out_vec, u);
-              else la_store4<T>(out + m * g.out_ld + n, left, g.out_vec, u);
-            }
+          for (int e = 0; e < 4; ++e) u[e] = acc[i][j][e] + b4[e];
+          if (g.z) {
+            if (g.z_f32) la_store4<float>(reinterpret_cast<float*>(g.z) + m * g.n + n, left, g.z_vec, u);
+            else la_store4<T>(reinterpret_cast<T*>(g.z) + m * g.n + n, left, g.z_vec, u);
           }
-        } else {                                         // LA_DACT / LA_DNORM: res = gy
-          float k1 = 0.f, k2 = 0.f;
-          float d[NN][4];
+          if (!out) continue;
+          ro_act<P, 4>(u, g.act);
+          if (res) {
+            float r[4];
+            la_load4<T>(res + m * g.res_ld + n, left, g.res_vec, r);
 #pragma unroll
-          for (int j = 0; j < NN; ++j) {
-            const int64_t n = n0 + wn + j * 16 + q * 4;
-            const int left = (int)min((int64_t)4, g.n - n);
-            float z[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]}, w4[4] = {1.f, 1.f, 1.f, 1.f};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) d[j][e] = 0.f;
-            if (row_ok && left > 0) la_load4<T>(res + m * g.res_ld + n, left, g.res_vec, d[j]);
-            if constexpr (EPI == LA_DNORM) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                w4[e] = e < left ? ro_param(g.g, g.norm_dtype, n + e, 1.f) : 0.f;
-                z[e] = fmaf(z[e], w4[e], e < left ? ro_param(g.h, g.norm_dtype, n + e, 0.f) : 0.f);
-              }
-            }
-            ro_act_slope<P, 4>(d[j], z, g.act);
-            if constexpr (EPI == LA_DNORM) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                if (row_ok) {
-                  sg[j][e] = fmaf(d[j][e], acc[i][j][e], sg[j][e]);
-                  sh[j][e] += d[j][e];
-                }
-                d[j][e] *= w4[e];
-                k1 += d[j][e];
-                k2 = fmaf(d[j][e], acc[i][j][e], k2);
-              }
-            }
+            for (int e = 0; e < 4; ++e) u[e] += r[e];
           }
-          if constexpr (EPI == LA_DNORM) {
-            const float inv_n = 1.f / (float)g.n;
-            k1 = la_q_sum(k1) * inv_n;
-            k2 = la_q_sum(k2) * inv_n;
-          }
-#pragma unroll
-          for (int j = 0; j < NN; ++j) {
-            const int64_t n = n0 + wn + j * 16 + q * 4;
-            const int left = (int)min((int64_t)4, g.n - n);
-            if constexpr (EPI == LA_DNORM) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) d[j][e] = rstd * (d[j][e] - k1 - acc[i][j][e] * k2);
-            }
-            if (row_ok && left > 0) la_store4<T>(out + m * g.out_ld + n, left, g.out_vec, d[j]);
-          }
+          la_store4<T>(out + m * g.n + n, left, g.out_vec, u);
         }
       }
-    }
-  }
-  if constexpr (EPI == LA_DNORM) {
-    // per-lane sums over the workgroup's rows -> over the 16 lanes of a channel group -> over the wavefronts (LDS, in wave order)
-    float* red = reinterpret_cast<float*>(lds_a);
-    static_assert(TA::BYTES >= WM * BN * 2 * 4, "reduction buffer");
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < NN; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float a = ro_lane_sum<16>(sg[j][e]), b = ro_lane_sum<16>(sh[j][e]);
-        if (r16 == 0) {
-          red[(wave * 2 + 0) * BN + j * 16 + q * 4 + e] = a;
-          red[(wave * 2 + 1) * BN + j * 16 + q * 4 + e] = b;
-        }
-      }
-    __syncthreads();
-    float* slab = g.slabs + (int64_t)blockIdx.x * g.slab_stride;
-    for (int c = threadIdx.x; c < 2 * BN; c += kBlock) {
-      const int s = c / BN, n = c % BN;
-      if (n >= g.n) continue;
-      float a = 0.f;
-      for (int w = 0; w < WM; ++w) a += red[(w * 2 + s) * BN + n];
-      slab[(int64_t)s * g.n + n] = a;
     }
   }
 }
@@ -438,34 +315,5 @@ template <typename T, int MA, int MB, int EPI> static int la_any(const LaArgs& a
   if (a.n > 64 && a.m > 64 && count(128, 128) >= 256) return la_go<T, MA, MB, 128, 128, 2, 2, EPI>(a, kLaGrid, st);
   return la_go<T, MA, MB, 64, 64, 2, 2, EPI>(a, kLaGrid, st);
 }
-
-// A norm needs all N channels of a row in one workgroup: N <= 256
-constexpr int kLaNormMax = 256;
-constexpr int kLaNormGrid = 1024;       // LA_DNORM: every workgroup writes a slab
-template <typename T, int EPI> static int la_norm_pick(const LaArgs& a, hipStream_t st, int* slabs) {
-  const int cap = EPI == LA_DNORM ? kLaNormGrid : kLaGrid;
-  // (the gradient's tile does not depend on the row count: a capacity-sized launch must cut the rows as an exactly sized one does)
-  const int bm = a.n > 128 || EPI == LA_DNORM || a.m <= 128 * 256 ? 64 : 128;
-  if (slabs) *slabs = (int)std::min<int64_t>((ceil_div(a.m, bm) + 7) / 8 * 8, cap);
-  if (a.n > 128) return la_go<T, LA_ROWS, LA_ROWS, 64, 256, 4, 1, EPI>(a, cap, st);
-  if (a.n > 64) return bm == 128 ? la_go<T, LA_ROWS, LA_ROWS, 128, 128, 4, 1, EPI>(a, cap, st) : la_go<T, LA_ROWS, LA_ROWS, 64, 128, 4, 1, EPI>(a, cap, st);
-  return bm == 128 ? la_go<T, LA_ROWS, LA_ROWS, 128, 64, 4, 1, EPI>(a, cap, st) : la_go<T, LA_ROWS, LA_ROWS, 64, 64, 4, 1, EPI>(a, cap, st);
-}
-
-// one translation unit per storage type (linear_f32.hip, ..) instantiates these
-template <typename T> int la_forward(const LaArgs& a, int norm, hipStream_t st);
-template <typename T> int la_dz(const LaArgs& a, int norm, hipStream_t st, int* slabs);
-template <typename T> int la_dx(const LaArgs& a, hipStream_t st);
-template <typename T> int la_dw(const LaArgs& a, hipStream_t st);
-
-#define PYGHO_LINEAR_TYPE(T)                                                                                              \
-  template <> int la_forward<T>(const LaArgs& a, int norm, hipStream_t st) {                                              \
-    return norm ? la_norm_pick<T, LA_NORM>(a, st, nullptr) : la_any<T, LA_ROWS, LA_ROWS, LA_ACT>(a, st);                  \
-  }                                                                                                                       \
-  template <> int la_dz<T>(const LaArgs& a, int norm, hipStream_t st, int* slabs) {                                       \
-    return norm ? la_norm_pick<T, LA_DNORM>(a, st, slabs) : la_any<T, LA_ROWS, LA_ROWS, LA_DACT>(a, st);                  \
-  }                                                                                                                       \
-  template <> int la_dx<T>(const LaArgs& a, hipStream_t st) { return la_any<T, LA_ROWS, LA_COLS, LA_ACT>(a, st); }        \
-  template <> int la_dw<T>(const LaArgs& a, hipStream_t st) { return la_any<T, LA_COLS, LA_COLS, LA_SLAB>(a, st); }
 
 }  // namespace pygho

@@ -114,4 +114,19 @@ template <int L> __device__ __forceinline__ float ro_lane_sum(float v) {
   return v;
 }
 
+// ---- shared launches (layer_norm.hip) -------------------------------------------------------------------------------------------------
+bool ro_float(int dtype);
+// the norm / activation of rows kept in `x_dtype` (dtype or f32), see pygho_layer_norm_act; sums = 3 (gg, gh, column sums of gx), 2 (gg, gh) or
+// 1 (no norm: gx = gy act'(x) and its column sums)
+int ln_fwd_launch(void* y, const void* x, int64_t x_ld, const void* weight, const void* bias, int param_dtype, const void* residual,
+                  int64_t residual_ld, int64_t m, int64_t c, float eps, int act, int dtype, int x_dtype, hipStream_t st);
+int64_t ln_bwd_slab_floats(int64_t m, int64_t c, int sums);
+int ln_bwd_launch(void* gx, float* slabs, int64_t* stride, int* n_slabs, int sums, const void* x, int64_t x_ld, const void* gy, int64_t gy_ld,
+                  const void* weight, const void* bias, int param_dtype, int64_t m, const int32_t* m_dev, int64_t c, float eps, int act, int dtype,
+                  int x_dtype, hipStream_t st);
+// out.p[0][0 .. len[0]) | out.p[1][..] | .. = the columns of n_slabs slabs (`stride` floats apart, a multiple of 4) added in a fixed order that
+// trailing slabs of zeros do not change; null outputs are skipped
+struct FoldOut { void* p[4]; int64_t len[4]; int dt[4]; };
+int fold_launch(const FoldOut& out, const float* slabs, int64_t n_slabs, int64_t stride, hipStream_t st);
+
 }  // namespace pygho

@@ -10,7 +10,6 @@ stored in x's dtype or (master weights) in f32; their gradients come back in the
 """
 from __future__ import annotations
 
-from ctypes import byref, c_int
 from typing import Optional, Tuple
 
 import torch
@@ -19,6 +18,7 @@ from torch.autograd.function import once_differentiable
 
 from ._native import DTYPE_CODE, check, lib, ptr, require_device, stream_ptr
 
+from .blocks import param_as
 from .plans import dyn_rows
 
 ROW_ACT_CODE = {"none": 0, "relu": 1, "silu": 2, "elu": 3}      # enum pygho_row_act
@@ -66,66 +66,51 @@ def _norm_params(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor]):
     return w, b, DTYPE_CODE[dt]
 
 
-def _layer_norm_fwd(x: Tensor, w, b, pdt: int, eps: float, act: str, residual: Optional[Tensor], out_shape, dtype: torch.dtype) -> Tensor:
-    c = x.shape[-1]
-    x2, x_ld = _rows(x, c)
-    r2, r_ld = _rows(residual, c)
-    y = torch.empty(out_shape, dtype=dtype, device=x.device)
-    check(lib().pygho_layer_norm_act(ptr(y), ptr(x2), x_ld, ptr(w), ptr(b), pdt, ptr(r2), r_ld, x2.shape[0], c, float(eps), ROW_ACT_CODE[act],
-                                     DTYPE_CODE[dtype], DTYPE_CODE[x2.dtype], stream_ptr(x.device)), "layer_norm_act")
-    return y
+def _workspace(nbytes: int, dev) -> Optional[Tensor]:
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
 
 
-def fold_partials(slabs: Tensor, n_slabs: int, stride: int, outs) -> None:
-    """add the columns of the first n_slabs f32 slabs into `outs`: up to four (tensor or None, length)"""
-    args = []
-    for k in range(4):
-        t, n = outs[k] if k < len(outs) else (None, 0)
-        args += [ptr(t), n, 0 if t is None else DTYPE_CODE[t.dtype]]
-    check(lib().pygho_fold_partials(*args, ptr(slabs), n_slabs, stride, stream_ptr(slabs.device)), "fold_partials")
-
-
-def _layer_norm_bwd(x: Tensor, gy: Tensor, w, b, pdt: int, eps: float, act: str, out_dtypes, want_colsum: bool = False):
-    """(gx (rows, c) in gy's dtype, gradients of weight, bias and the column sums of gx in `out_dtypes`; None where that is None)"""
-    c = x.shape[-1]
-    x2, x_ld = _rows(x, c)
-    gy2, gy_ld = _rows(gy, c)
-    m, dev = x2.shape[0], x2.device
-    sums = 3 if want_colsum else 2
-    stride = (sums * c + 3) // 4 * 4
-    gx = torch.empty((m, c), dtype=gy2.dtype, device=dev)
-    slabs = torch.empty((max(1, int(lib().pygho_layer_norm_act_bwd_slabs(m))), stride), dtype=torch.float32, device=dev)
-    n = c_int(0)
-    check(lib().pygho_layer_norm_act_bwd(ptr(gx), ptr(slabs), stride, sums, byref(n), ptr(x2), x_ld, ptr(gy2), gy_ld, ptr(w), ptr(b), pdt, m,
-                                         ptr(dyn_rows(m)), c, float(eps), ROW_ACT_CODE[act], DTYPE_CODE[gy2.dtype], DTYPE_CODE[x2.dtype],
-                                         stream_ptr(dev)), "layer_norm_act_bwd")
-    outs = [None if d is None else torch.empty(c, dtype=d, device=dev) for d in out_dtypes]
-    if any(o is not None for o in outs):
-        fold_partials(slabs, n.value, stride, [(o, c) for o in outs[:sums]])
-    return (gx,) + tuple(outs)
+def _grad(need: bool, shape, dtype, dev):
+    """(tensor or None, address, dtype code) of a parameter's gradient"""
+    if not need:
+        return None, None, 0
+    t = torch.empty(shape, dtype=dtype, device=dev)
+    return t, t.data_ptr(), DTYPE_CODE[dtype]
 
 
 class _LayerNormAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, eps, act):
         w, b, pdt = _norm_params(x, weight, bias)
-        xs = x if x.dim() == 2 and (x.stride(1) == 1 or x.shape[1] == 1) else _rows(x, x.shape[-1])[0]
-        y = _layer_norm_fwd(xs, w, b, pdt, eps, act, residual, x.shape, x.dtype)
-        ctx.save_for_backward(xs, w, b)
-        ctx.meta = (pdt, eps, act, x.shape, None if weight is None else weight.dtype, None if bias is None else bias.dtype)
+        c = x.shape[-1]
+        x2, x_ld = _rows(x, c)
+        r2, r_ld = _rows(residual, c)
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        check(lib().pygho_layer_norm_act(ptr(y), ptr(x2), x_ld, ptr(w), ptr(b), pdt, ptr(r2), r_ld, x2.shape[0], c, float(eps), ROW_ACT_CODE[act],
+                                         DTYPE_CODE[x.dtype], stream_ptr(x.device)), "layer_norm_act")
+        ctx.save_for_backward(x2, w, b)
+        ctx.meta = (x_ld, pdt, eps, act, x.shape, None if weight is None else weight.dtype, None if bias is None else bias.dtype)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gy):
-        xs, w, b = ctx.saved_tensors
-        pdt, eps, act, shape, w_dtype, b_dtype = ctx.meta
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        gx = gw = gb = None
-        if need_x or need_w or need_b:
-            gx, gw, gb = _layer_norm_bwd(xs, gy, w, b, pdt, eps, act, (w_dtype if need_w else None, b_dtype if need_b else None))
-            gx = gx.view(shape) if need_x else None
-        return gx, gw, gb, (gy if need_r else None), None, None
+        if not (need_x or need_w or need_b):
+            return None, None, None, (gy if need_r else None), None, None
+        x2, w, b = ctx.saved_tensors
+        x_ld, pdt, eps, act, shape, w_dtype, b_dtype = ctx.meta
+        (m, c), dev, code = x2.shape, x2.device, DTYPE_CODE[x2.dtype]
+        gy2, gy_ld = _rows(gy, c)
+        gx = torch.empty(shape, dtype=x2.dtype, device=dev)
+        gw, gw_ptr, gw_code = _grad(need_w, c, w_dtype, dev)
+        gb, gb_ptr, gb_code = _grad(need_b, c, b_dtype, dev)
+        nbytes = int(lib().pygho_layer_norm_act_bwd_workspace(m, c))
+        ws = _workspace(nbytes, dev)
+        check(lib().pygho_layer_norm_act_bwd(ptr(gx), gw_ptr, gw_code, gb_ptr, gb_code, ptr(x2), x_ld, ptr(gy2), gy_ld, ptr(w), ptr(b), pdt, m,
+                                             ptr(dyn_rows(m)), c, float(eps), ROW_ACT_CODE[act], code, ptr(ws), nbytes, stream_ptr(dev)),
+              "layer_norm_act_bwd")
+        return (gx if need_x else None), gw, gb, (gy if need_r else None), None, None
 
 
 def layer_norm_act(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5, act: str = "none",
@@ -162,96 +147,54 @@ def _bias(b: Optional[Tensor], dtype: torch.dtype):
     return b.contiguous(), DTYPE_CODE[b.dtype]
 
 
-def _linear_fwd(x2: Tensor, x_ld: int, w: Tensor, w_ld: int, b, bdt: int, norm, eps: float, act: str, residual: Optional[Tensor], out_shape,
-                out_dtype: torch.dtype) -> Tensor:
-    """norm: None, or (g, h, dtype code)"""
-    n, k = w.shape
-    r2, r_ld = _rows(residual, n)
-    y = torch.empty(out_shape, dtype=out_dtype, device=x2.device)
-    g, h, pdt = norm if norm is not None else (None, None, 0)
-    check(lib().pygho_linear_act(ptr(y), ptr(x2), x_ld, ptr(w), w_ld, ptr(b), bdt, 0 if norm is None else 1, ptr(g), ptr(h), pdt, float(eps),
-                                 ptr(r2), r_ld, x2.shape[0], k, n, ROW_ACT_CODE[act], DTYPE_CODE[x2.dtype], DTYPE_CODE[out_dtype],
-                                 stream_ptr(x2.device)), "linear_act")
-    return y
-
-
 class _LinearAct(torch.autograd.Function):
-    """act([LayerNorm](x W^T + b) [* g + h]) + residual.  What backward reads: x and the parameters; the product itself is formed again, except
-    behind a norm over more channels than one workgroup holds (pygho_linear_norm_max), where it is kept in f32."""
+    """act([LayerNorm](x W^T + b) [* g + h]) + residual.  Kept for backward: x, the parameters and, where the C side says so
+    (pygho_linear_act_keeps: W does not fit a CU's LDS), the pre-activation."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, g, h, residual, eps, act, normed):
-        from .blocks import param_as
-        dt = x.dtype
+        dt, dev = x.dtype, x.device
         n, k = weight.shape
         w, w_ld = _matrix(param_as(weight, dt).detach())
         b, bdt = _bias(bias, dt)
         x2, x_ld = _rows(x, k)
-        norm = None
-        if normed:
-            norm = _norm_params(x, g, h)
-        out_shape = tuple(x.shape[:-1]) + (n,)
+        r2, r_ld = _rows(residual, n)
+        gg, hh, pdt = _norm_params(x, g, h) if normed else (None, None, 0)
+        m, code = x2.shape[0], DTYPE_CODE[dt]
+        y = torch.empty(tuple(x.shape[:-1]) + (n,), dtype=dt, device=dev)
+        keeps = int(lib().pygho_linear_act_keeps(k, n, int(normed), ROW_ACT_CODE[act], code))
         z = None
-        if normed and n > int(lib().pygho_linear_norm_max()):
-            z = _linear_fwd(x2, x_ld, w, w_ld, b, bdt, None, 0.0, "none", None, (x2.shape[0], n), torch.float32)
-            y = _layer_norm_fwd(z, norm[0], norm[1], norm[2], eps, act, residual, out_shape, dt)
-        else:
-            y = _linear_fwd(x2, x_ld, w, w_ld, b, bdt, norm, eps, act, residual, out_shape, dt)
-        ctx.save_for_backward(x2, w, b, z, *(norm[:2] if normed else (None, None)))
-        ctx.meta = (bdt, norm[2] if normed else 0, eps, act, normed, x.shape, weight.dtype,
-                    *(None if t is None else t.dtype for t in (bias, g, h)))
+        if keeps == 2 or (keeps == 1 and any(ctx.needs_input_grad[:5])):
+            z = torch.empty((m, n), dtype=torch.float32 if keeps == 2 else dt, device=dev)
+        check(lib().pygho_linear_act(ptr(y), ptr(z), ptr(x2), x_ld, ptr(w), w_ld, ptr(b), bdt, int(normed), ptr(gg), ptr(hh), pdt, float(eps),
+                                     ptr(r2), r_ld, m, k, n, ROW_ACT_CODE[act], code, stream_ptr(dev)), "linear_act")
+        ctx.save_for_backward(x2, w, b, z, gg, hh)
+        ctx.meta = (x_ld, w_ld, bdt, pdt, eps, act, normed, x.shape, weight.dtype, *(None if t is None else t.dtype for t in (bias, g, h)))
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gy):
-        x2, w, b, z, g, h = ctx.saved_tensors
-        bdt, pdt, eps, act, normed, x_shape, w_dtype, b_dtype, g_dtype, h_dtype = ctx.meta
         need_x, need_w, need_b, need_g, need_h, need_r = ctx.needs_input_grad[:6]
-        out = [None] * 6
-        out[5] = gy if need_r else None
+        res = gy if need_r else None
         if not (need_x or need_w or need_b or need_g or need_h):
-            return (*out, None, None, None)
+            return None, None, None, None, None, res, None, None, None
+        x2, w, b, z, g, h = ctx.saved_tensors
+        x_ld, w_ld, bdt, pdt, eps, act, normed, x_shape, w_dtype, b_dtype, g_dtype, h_dtype = ctx.meta
         n, k = w.shape
-        w, w_ld = _matrix(w)
-        x2, x_ld = _rows(x2, k)
         gy2, gy_ld = _rows(gy, n)
-        m, dev, dt = x2.shape[0], x2.device, x2.dtype
-        st, code, m_dev = stream_ptr(dev), DTYPE_CODE[dt], dyn_rows(m)
-        if z is not None:
-            dz, out[3], out[4], out[2] = _layer_norm_bwd(z, gy2, g, h, pdt, eps, act, (g_dtype if need_g else None, h_dtype if need_h else None,
-                                                                                       b_dtype if need_b else None), want_colsum=True)
-            dz_ld = n
-        elif act == "none" and not normed:
-            dz, dz_ld = gy2, gy_ld
-        else:
-            dz, dz_ld = torch.empty((m, n), dtype=dt, device=dev), n
-            stride = (2 * n + 3) // 4 * 4
-            slabs = torch.empty((max(1, int(lib().pygho_linear_act_dz_slabs(m))), stride), dtype=torch.float32, device=dev) if normed else None
-            used = c_int(0)
-            check(lib().pygho_linear_act_dz(ptr(dz), ptr(slabs), stride, byref(used), ptr(x2), x_ld, ptr(w), w_ld, ptr(b), bdt, 1 if normed else 0,
-                                            ptr(g), ptr(h), pdt, float(eps), ptr(gy2), gy_ld, m, ptr(m_dev), k, n, ROW_ACT_CODE[act], code, st),
-                  "linear_act_dz")
-            if need_g or need_h:
-                out[3] = torch.empty(n, dtype=g_dtype, device=dev) if need_g else None
-                out[4] = torch.empty(n, dtype=h_dtype, device=dev) if need_h else None
-                fold_partials(slabs, used.value, stride, [(out[3], n), (out[4], n)])
-        if need_x:
-            gx = torch.empty((m, k), dtype=dt, device=dev)
-            check(lib().pygho_linear_dx(ptr(gx), ptr(dz), dz_ld, ptr(w), w_ld, m, k, n, code, st), "linear_dx")
-            out[0] = gx.view(x_shape)
-        if need_w or (need_b and out[2] is None):
-            colsum = need_b and out[2] is None
-            count = int(lib().pygho_linear_dw_slabs(m, k, n))
-            stride = (n * k + (n if colsum else 0) + 3) // 4 * 4
-            slabs = torch.empty((max(1, count), stride), dtype=torch.float32, device=dev)
-            check(lib().pygho_linear_dw(ptr(slabs), stride, ptr(dz), dz_ld, ptr(x2), x_ld, m, ptr(m_dev), k, n, 1 if colsum else 0, code, st),
-                  "linear_dw")
-            out[1] = torch.empty((n, k), dtype=w_dtype, device=dev) if need_w else None
-            if colsum:
-                out[2] = torch.empty(n, dtype=b_dtype, device=dev)
-            fold_partials(slabs, count, stride, [(out[1], n * k), (out[2] if colsum else None, n if colsum else 0)])
-        return (*out, None, None, None)
+        m, dev, code = x2.shape[0], x2.device, DTYPE_CODE[x2.dtype]
+        gx = torch.empty(x_shape, dtype=x2.dtype, device=dev) if need_x else None
+        gw, gw_ptr, gw_code = _grad(need_w, (n, k), w_dtype, dev)
+        gb, gb_ptr, gb_code = _grad(need_b, n, b_dtype, dev)
+        gg, gg_ptr, gg_code = _grad(need_g, n, g_dtype, dev)
+        gh, gh_ptr, gh_code = _grad(need_h, n, h_dtype, dev)
+        nbytes = int(lib().pygho_linear_act_bwd_workspace(m, k, n, int(normed), ROW_ACT_CODE[act], code))
+        ws = _workspace(nbytes, dev)
+        check(lib().pygho_linear_act_bwd(ptr(gx), gw_ptr, gw_code, gb_ptr, gb_code, gg_ptr, gg_code, gh_ptr, gh_code, ptr(z), ptr(x2), x_ld, ptr(w),
+                                         w_ld, ptr(b), bdt, int(normed), ptr(g), ptr(h), pdt, float(eps), ptr(gy2), gy_ld, m, ptr(dyn_rows(m)),
+                                         k, n, ROW_ACT_CODE[act], code, ptr(ws), nbytes, stream_ptr(dev)), "linear_act_bwd")
+        return gx, gw, gb, gg, gh, res, None, None, None
 
 
 def _linear_args(x: Tensor, weight: Tensor, bias: Optional[Tensor], act: str, residual: Optional[Tensor], what: str) -> None:
@@ -268,8 +211,8 @@ def _linear_args(x: Tensor, weight: Tensor, bias: Optional[Tensor], act: str, re
 
 def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: str = "none", residual: Optional[Tensor] = None) -> Tensor:
     """act(x @ weight^T + bias) + residual over the last dim of x in one launch; act is one of "none", "relu", "silu", "elu".  weight (N, K) and
-    bias (N,): in x's dtype, or f32 master parameters (the product then takes their copy in x's dtype, `param_as`), residual: the output's
-    shape and x's dtype.  Backward: the gradient of the pre-activation (formed again from x), dX and dW / db on the same tiled product."""
+    bias (N,): in x's dtype, or f32 master parameters (the product then takes W's copy in x's dtype, `param_as`), residual: the output's shape and
+    x's dtype."""
     _linear_args(x, weight, bias, act, residual, "linear_act")
     return _LinearAct.apply(x, weight, bias, None, None, residual, 0.0, act, False)
 
@@ -277,8 +220,8 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: st
 def linear_norm_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, norm_weight: Optional[Tensor] = None,
                     norm_bias: Optional[Tensor] = None, eps: float = 1e-5, act: str = "none", residual: Optional[Tensor] = None) -> Tensor:
     """act(LayerNorm(x @ weight^T + bias) * norm_weight + norm_bias) + residual: one [Linear, LayerNorm, act] block of an MLP with the layer's
-    residual connection.  Up to 256 output channels in one launch (the pre-activation never reaches memory), beyond that the product in f32
-    and `layer_norm_act` over it.  Arguments as in `linear_act` and `layer_norm_act`."""
+    residual connection.  One launch where W fits a CU's LDS (up to 256 output channels; the pre-activation never reaches memory), otherwise the
+    product in f32 and the norm over it.  Arguments as in `linear_act` and `layer_norm_act`."""
     what = "linear_norm_act"
     _linear_args(x, weight, bias, act, residual, what)
     n = weight.shape[0]
