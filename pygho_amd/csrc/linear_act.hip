@@ -4,10 +4,12 @@
 namespace pygho {
 
 #define PYGHO_LINEAR_DECL(T)                                                                  \
-  template <> bool LinearOps<T>::stream_fits(int64_t, int64_t, int);                          \
-  template <> bool LinearOps<T>::stream_dx_fits(int64_t, int64_t, int);                       \
+  template <> int LinearOps<T>::stream_lds(int64_t, int64_t, int, bool, bool);                \
+  template <> int LinearOps<T>::out_lds(int64_t, int64_t);                                    \
+  template <> bool LinearOps<T>::dw_fits(int64_t, int64_t, int);                              \
   template <> int LinearOps<T>::stream_fwd(const LsArgs&, int, hipStream_t);                  \
-  template <> int LinearOps<T>::stream_bwd(const LsArgs&, int, int*, hipStream_t);            \
+  template <> int LinearOps<T>::out_fwd(const LsArgs&, hipStream_t);                          \
+  template <> int LinearOps<T>::stream_bwd(const LsArgs&, int, bool, int*, hipStream_t);      \
   template <> int LinearOps<T>::tile_act(const LaArgs&, hipStream_t);                         \
   template <> int LinearOps<T>::tile_dx(const LaArgs&, hipStream_t);                          \
   template <> int LinearOps<T>::tile_dw(const LaArgs&, hipStream_t);
@@ -41,9 +43,17 @@ static int la_stride_check(const char* what, int64_t a, int64_t b, int dtype) { 
 }
 static LaOperand la_operand(const void* p, int64_t ld, int dtype) { return LaOperand{p, ld, la_aligned(p, ld, la_size(dtype), 16) ? 1 : 0}; }
 
-// the form of an operator over (k, n): W in LDS, or tiles
-static bool la_streams(int64_t k, int64_t n, int norm, int dtype) {
-  return la_type(dtype, [&](auto ops) { return ops.stream_fits(k, n, norm); });
+// The form of a forward over (k, n).  W fits a CU's LDS: linear_stream.h where a norm needs the row, for narrow outputs (linear_out.h forms 64
+// channels at a time) and for k beyond what linear_out.h holds in registers; linear_out.h for the rest.  Otherwise tiles
+enum { FORM_TILE = 0, FORM_STREAM = 1, FORM_OUT = 2 };
+static int la_form(int64_t k, int64_t n, int norm, int dtype) {
+  return la_type(dtype, [&](auto ops) {
+    const bool stream = ops.stream_lds(k, n, 0, false, false) <= kLsLds, out = !norm && ops.out_lds(k, n) <= kLsLds;
+    return stream && (!out || n <= 32) ? FORM_STREAM : out ? FORM_OUT : FORM_TILE;
+  });
+}
+static int la_forward(const LsArgs& a, int form, int norm, int dtype, hipStream_t st) {
+  return la_type(dtype, [&](auto ops) { return form == FORM_OUT ? ops.out_fwd(a, st) : ops.stream_fwd(a, norm, st); });
 }
 static LsArgs la_stream_args(const void* x, int64_t x_ld, const void* w, int64_t w_ld, const void* bias, int bias_dtype, const void* g, const void* h,
                              int norm_dtype, const void* r, int64_t r_ld, void* out, int64_t m, int64_t k, int64_t n, double eps, int act, int dtype) {
@@ -54,7 +64,7 @@ static LsArgs la_stream_args(const void* x, int64_t x_ld, const void* w, int64_t
   a.bias = bias; a.bias_dtype = bias_dtype; a.g = g; a.h = h; a.norm_dtype = norm_dtype;
   a.r = r; a.r_ld = r_ld;
   a.out = out;
-  a.vec = k % (64 / es) == 0 && n % 16 == 0 && la_aligned(x, x_ld, es, 16) && la_aligned(r, r_ld, es, 4 * es) && la_aligned(out, n, es, 4 * es);
+  a.vec = (k % (64 / es) == 0 && la_aligned(x, x_ld, es, 16) ? 1 : 0) | (n % 16 == 0 && la_aligned(r, r_ld, es, 4 * es) && la_aligned(out, n, es, 4 * es) ? 2 : 0);
   a.m = m; a.k = (int)k; a.n = (int)n; a.eps = (float)eps; a.act = act;
   return a;
 }
@@ -81,17 +91,23 @@ static int64_t la_dw_slabs(int64_t m, int64_t k, int64_t n) {
 }
 static int64_t la_pad4(int64_t v) { return (v + 3) / 4 * 4; }
 
-// workspace of a backward pass, in bytes: [dz (16-byte padded)] [z] [slabs of the sums over n] [slabs of dW | db].
-// z: a forward that streams has not kept the pre-activation; where its backward is too wide to stream, z is formed again in f32 for the row kernel
-struct LaSpace { int64_t dz, z, sums, dw, total; int nsum; bool stream, own_dz; };
-static LaSpace la_space(int64_t m, int64_t k, int64_t n, int norm, int act, int dtype) {
+// The launches of a backward pass and its workspace, in bytes: [dz] [z] [slabs of the sums over n] [slabs of dW | db]
+//   fused   dz, dX, dW and every sum from one streaming launch (operands aligned; its slabs are [sums | dW])
+//   stream  dz with the sums (and dX where both copies of W fit) from a streaming launch
+//   else    dz by the row kernel from the pre-activation: kept by the forward, or (z) formed again in f32 where the forward streams
+struct LaSpace { int64_t dz, z, sums, dw, total; int nsum; bool fused, stream, own_dz; };
+static LaSpace la_space(int64_t m, int64_t k, int64_t n, int norm, int act, int dtype, bool aligned) {
   LaSpace s{};
-  const bool fwd_streams = la_streams(k, n, norm, dtype);
-  s.stream = fwd_streams && n <= ls_bwd_max(norm);
   s.nsum = norm ? 3 : 1;
+  s.fused = aligned && la_type(dtype, [&](auto ops) { return ops.dw_fits(k, n, s.nsum); });
+  if (s.fused) {
+    s.total = s.dw = kLsGrid * la_pad4(s.nsum * n + n * k) * 4;
+    return s;
+  }
   s.own_dz = norm || act != kActNone;
+  s.stream = s.own_dz && n <= ls_bwd_max(norm) && la_type(dtype, [&](auto ops) { return ops.stream_lds(k, n, s.nsum, false, false) <= kLsLds; });
   s.dz = s.own_dz ? (m * n * la_size(dtype) + 15) / 16 * 16 : 0;
-  s.z = s.own_dz && fwd_streams && !s.stream ? (m * n * 4 + 15) / 16 * 16 : 0;
+  s.z = s.own_dz && !s.stream && la_form(k, n, norm, dtype) != FORM_TILE ? (m * n * 4 + 15) / 16 * 16 : 0;
   s.sums = !s.own_dz ? 0 : s.stream ? kLsGrid * la_pad4(s.nsum * n) * 4 : ln_bwd_slab_floats(m, n, s.nsum) * 4;
   s.dw = la_dw_slabs(m, k, n) * la_pad4(n * k + n) * 4;
   s.total = s.dz + s.z + s.sums + s.dw;
@@ -105,7 +121,7 @@ using namespace pygho;
 // what the forward keeps for the backward besides x: 0 nothing, 1 the pre-activation in the rows' type, 2 the pre-activation in f32 (needed by the
 // forward itself as well)
 extern "C" int pygho_linear_act_keeps(int64_t k, int64_t n, int norm, int act, int dtype) {
-  if (k <= 0 || n <= 0 || !ro_float(dtype) || la_streams(k, n, norm, dtype)) return 0;
+  if (k <= 0 || n <= 0 || !ro_float(dtype) || la_form(k, n, norm, dtype) != FORM_TILE) return 0;
   return norm ? 2 : act != kActNone ? 1 : 0;
 }
 
@@ -119,10 +135,8 @@ extern "C" int pygho_linear_act(void* y, void* z, const void* x, int64_t x_ld, c
   if (m == 0) return PYGHO_OK;
   if (!y || !x || !w) { set_error("null pointer"); return PYGHO_ERR_INVALID; }
   hipStream_t st = (hipStream_t)stream;
-  if (la_streams(k, n, norm, dtype)) {
-    const LsArgs a = la_stream_args(x, x_ld, w, w_ld, bias, bias_dtype, g, h, norm_dtype, residual, residual_ld, y, m, k, n, eps, act, dtype);
-    return la_type(dtype, [&](auto ops) { return ops.stream_fwd(a, norm, st); });
-  }
+  if (const int form = la_form(k, n, norm, dtype); form != FORM_TILE)
+    return la_forward(la_stream_args(x, x_ld, w, w_ld, bias, bias_dtype, g, h, norm_dtype, residual, residual_ld, y, m, k, n, eps, act, dtype), form, norm, dtype, st);
   if (!norm) return la_tile_act(x, x_ld, w, w_ld, bias, bias_dtype, residual, residual_ld, y, z, 0, m, k, n, act, dtype, st);
   if (!z) { set_error("linear_act: this norm needs the pre-activation's buffer (pygho_linear_act_keeps)"); return PYGHO_ERR_INVALID; }
   if (int rc = la_tile_act(x, x_ld, w, w_ld, bias, bias_dtype, nullptr, 0, nullptr, z, 1, m, k, n, kActNone, dtype, st)) return rc;
@@ -131,7 +145,7 @@ extern "C" int pygho_linear_act(void* y, void* z, const void* x, int64_t x_ld, c
 
 extern "C" size_t pygho_linear_act_bwd_workspace(int64_t m, int64_t k, int64_t n, int norm, int act, int dtype) {
   if (m <= 0 || k <= 0 || n <= 0 || !ro_float(dtype)) return 0;
-  return (size_t)la_space(m, k, n, norm, act, dtype).total;
+  return (size_t)std::max(la_space(m, k, n, norm, act, dtype, true).total, la_space(m, k, n, norm, act, dtype, false).total);
 }
 
 extern "C" int pygho_linear_act_bwd(void* gx, void* gw, int gw_dtype, void* gb, int gb_dtype, void* gg, int gg_dtype, void* gh, int gh_dtype,
@@ -147,17 +161,32 @@ extern "C" int pygho_linear_act_bwd(void* gx, void* gw, int gw_dtype, void* gb, 
     return PYGHO_ERR_UNSUPPORTED;
   }
   if (int rc = la_stride_check("linear_act_bwd", x_ld, gy_ld, dtype)) return rc;
-  const LaSpace sp = la_space(m_cap, k, n, norm, act, dtype);
   hipStream_t st = (hipStream_t)stream;
   if (m_cap == 0) {                                           // no rows: every gradient of a parameter is zero
     if (int rc = fold_launch(FoldOut{{gw, gb, gg, gh}, {gw ? n * k : 0, gb ? n : 0, gg ? n : 0, gh ? n : 0}, {gw_dtype, gb_dtype, gg_dtype, gh_dtype}}, nullptr, 0, 0, st)) return rc;
     return PYGHO_OK;
   }
   if (!x || !w || !gy || !workspace) { set_error("null pointer"); return PYGHO_ERR_INVALID; }
-  if (workspace_bytes < (size_t)sp.total || (uintptr_t)workspace % 16 != 0) { set_error("linear_act_bwd: workspace too small or not 16-byte aligned"); return PYGHO_ERR_INVALID; }
-  if (pygho_linear_act_keeps(k, n, norm, act, dtype) != 0 && !z) { set_error("linear_act_bwd: the kept pre-activation is missing"); return PYGHO_ERR_INVALID; }
   const int es = la_size(dtype);
   char* base = reinterpret_cast<char*>(workspace);
+  // (`out`: dz's place, aligned by its own rule; gx joins the condition because dX is stored in the same launch)
+  LsArgs fa = la_stream_args(x, x_ld, w, w_ld, bias, bias_dtype, g, h, norm_dtype, gy, gy_ld, base, m_cap, k, n, eps, act, dtype);
+  if (gx && !(k % 16 == 0 && la_aligned(gx, k, es, 4 * es))) fa.vec &= 1;
+  fa.m_dev = m_dev;
+  const LaSpace sp = la_space(m_cap, k, n, norm, act, dtype, fa.vec == 3);
+  if (workspace_bytes < (size_t)sp.total || (uintptr_t)workspace % 16 != 0) { set_error("linear_act_bwd: workspace too small or not 16-byte aligned"); return PYGHO_ERR_INVALID; }
+  if (pygho_linear_act_keeps(k, n, norm, act, dtype) != 0 && !z) { set_error("linear_act_bwd: the kept pre-activation is missing"); return PYGHO_ERR_INVALID; }
+  if (sp.fused) {
+    fa.out = nullptr;
+    fa.gx = gx;
+    fa.slabs = reinterpret_cast<float*>(base);
+    fa.slab_stride = la_pad4(sp.nsum * n + n * k);
+    int used = 0;
+    if (int rc = la_type(dtype, [&](auto ops) { return ops.stream_bwd(fa, norm, true, &used, st); })) return rc;
+    const FoldOut o = norm ? FoldOut{{gg, gh, gb, gw}, {n, n, n, n * k}, {gg_dtype, gh_dtype, gb_dtype, gw_dtype}}
+                           : FoldOut{{gb, gw, nullptr, nullptr}, {n, n * k, 0, 0}, {gb_dtype, gw_dtype, 0, 0}};
+    return gb || gg || gh || gw ? fold_launch(o, fa.slabs, used, fa.slab_stride, st) : PYGHO_OK;
+  }
   const void* dz = gy;
   int64_t dz_ld = gy_ld;
   bool have_gx = gx == nullptr;
@@ -167,20 +196,17 @@ extern "C" int pygho_linear_act_bwd(void* gx, void* gw, int gw_dtype, void* gb, 
     int64_t stride = la_pad4(sp.nsum * n);
     int used = 0;
     if (sp.stream) {
-      LsArgs a = la_stream_args(x, x_ld, w, w_ld, bias, bias_dtype, g, h, norm_dtype, gy, gy_ld, own, m_cap, k, n, eps, act, dtype);
-      a.m_dev = m_dev;
-      a.slabs = slabs; a.slab_stride = stride;
-      if (gx && la_type(dtype, [&](auto ops) { return ops.stream_dx_fits(k, n, norm); })) {
-        a.gx = gx;
-        a.vec = a.vec && la_aligned(gx, k, es, 4 * es);
+      fa.slabs = slabs; fa.slab_stride = stride;
+      if (gx && la_type(dtype, [&](auto ops) { return ops.stream_lds(k, n, sp.nsum, true, false) <= kLsLds; })) {
+        fa.gx = gx;
         have_gx = true;
       }
-      if (int rc = la_type(dtype, [&](auto ops) { return ops.stream_bwd(a, norm, &used, st); })) return rc;
+      if (int rc = la_type(dtype, [&](auto ops) { return ops.stream_bwd(fa, norm, false, &used, st); })) return rc;
     } else {
       if (sp.z) {
         LsArgs a = la_stream_args(x, x_ld, w, w_ld, bias, bias_dtype, nullptr, nullptr, 0, nullptr, 0, base + sp.dz, m_cap, k, n, 0.0, kActNone, dtype);
         a.out_f32 = 1;
-        if (int rc = la_type(dtype, [&](auto ops) { return ops.stream_fwd(a, 0, st); })) return rc;
+        if (int rc = la_forward(a, la_form(k, n, 0, dtype), 0, dtype, st)) return rc;
         z = base + sp.dz;
       }
       if (int rc = ln_bwd_launch(own, slabs, &stride, &used, sp.nsum, z, n, gy, gy_ld, g, h, norm_dtype, m_cap, m_dev, n, (float)eps, act, dtype,
@@ -196,10 +222,10 @@ extern "C" int pygho_linear_act_bwd(void* gx, void* gw, int gw_dtype, void* gb, 
   }
   if (!have_gx) {
     // dX = dz . W: a product over n with k output channels
-    if (la_streams(n, k, 0, dtype)) {
+    if (const int form = la_form(n, k, 0, dtype); form != FORM_TILE) {
       LsArgs a = la_stream_args(dz, dz_ld, w, w_ld, nullptr, 0, nullptr, nullptr, 0, nullptr, 0, gx, m_cap, n, k, 0.0, kActNone, dtype);
       a.w_trans = 1;
-      if (int rc = la_type(dtype, [&](auto ops) { return ops.stream_fwd(a, 0, st); })) return rc;
+      if (int rc = la_forward(a, form, 0, dtype, st)) return rc;
     } else {
       LaArgs a{};
       a.a = la_operand(dz, dz_ld, dtype);

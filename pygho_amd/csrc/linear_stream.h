@@ -26,7 +26,7 @@ struct LsArgs {
   void* gx;                                                   // backward, nullable: dX (rows of k)
   float* slabs; int64_t slab_stride;                          // backward: LS_DACT [gb], LS_DNORM [gg | gh | gb]
   int64_t m; const int32_t* m_dev; int k; int n; float eps; int act;
-  int vec;                                                    // see VEC
+  int vec;                                                    // VEC of the kernels
   int red_bytes;                                              // bytes reserved for W and, at the end, for the reduction
 };
 
@@ -128,14 +128,20 @@ template <typename T, int NB> struct LsGeom {
   static constexpr int param_bytes = 4 * NP * 4;
 };
 
-// VEC: k is a whole number of 64-byte steps, n of 16 channels, and every row of x, r, out and gx allows 16-byte (x) / 4-element accesses.  A block's
-// rows then are one uniform base address, one 32-bit offset per lane and constants -- 64-bit addresses per access, or masks per element, take
-// more registers than the sums do.  Otherwise element by element
-template <typename T, int NB, int EPI, bool DX, bool VEC>
+// VEC & 1: k is a whole number of 64-byte steps and x's rows allow 16-byte accesses.  VEC & 2: n is a whole number of 16 channels and the rows of r, out
+// and gx allow accesses of 4 elements (k of 16, with gx).  A block's rows then are one uniform base address, one 32-bit offset per lane and
+// constants -- 64-bit addresses per access, or masks per element, take more registers than the sums do.  Otherwise element by element.
+//
+// DW (16-bit, k <= 128): the weight gradient in the same launch.  The workgroup's 8 wavefronts go through their blocks in step; each puts its dz
+// and its x (16 rows, row-major) into LDS, and after a barrier forms its share of dW += dz^T x over the 128 rows, both operands read back
+// transposed by the LDS (ds_read_b64_tr_b16).  dz never reaches memory and x is read once: 3 streams instead of 6
+template <typename T, int NB, int EPI, bool DX, int VEC, bool DW = false>
 __global__ __launch_bounds__(kLsThreads) void linear_stream_kernel(LsArgs a) {
   using G = LsGeom<T, NB>;
   constexpr bool P = Precise<T>::value, BWD = EPI == LS_DACT || EPI == LS_DNORM, NORM = EPI == LS_NORM || EPI == LS_DNORM;
   constexpr int ES = G::ES, E = 16 / ES, NP = G::NP, KC = 4;
+  constexpr bool XV = VEC & 1, NV = VEC & 2;
+  static_assert(!DW || (DX && BWD && ES == 2 && VEC == 3 && NB >= 4 && NB <= 8), "fused weight gradient");
   constexpr int NSUM = EPI == LS_DNORM ? 3 : EPI == LS_DACT ? 1 : 0;      // sums per channel
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int K = a.k, N = a.n, KS = G::steps(K), pitch = G::pitch_w(K);
@@ -221,11 +227,12 @@ __global__ __launch_bounds__(kLsThreads) void linear_stream_kernel(LsArgs a) {
   auto lane_row = [&](int64_t b) { return min(r16, (int)min((int64_t)15, m_rows - 1 - b * 16)); };
   uint4 xc[KC], xn[KC];
   auto load_x = [&](int64_t b, int kc, uint4 (&dst)[KC]) {
+    if (DW) b = min(b, n_blocks - 1);                          // (in step: a wavefront may be past the last block)
     const char* base = reinterpret_cast<const char*>(a.x) + b * 16 * a.x_ld * ES + kc * (KC * 64);
-    const uint32_t off = (uint32_t)lane_row(b) * (uint32_t)(a.x_ld * ES) + (VEC ? q * 16 : 0);
+    const uint32_t off = (uint32_t)lane_row(b) * (uint32_t)(a.x_ld * ES) + (XV ? q * 16 : 0);
 #pragma unroll
     for (int s = 0; s < KC; ++s) {
-      if constexpr (VEC) {
+      if constexpr (XV) {
         if (kc * KC + s < KS) dst[s] = *reinterpret_cast<const uint4*>(base + off + s * 64);
       } else {
         dst[s] = ls_load16<T>(reinterpret_cast<const T*>(base + off), s * (64 / ES) + q * E, K - kc * (KC * 64 / ES), 0);
@@ -233,8 +240,24 @@ __global__ __launch_bounds__(kLsThreads) void linear_stream_kernel(LsArgs a) {
     }
   };
   int64_t blk = (int64_t)blockIdx.x * waves + wave;
-  if (blk < n_blocks) load_x(blk, 0, xc);
-  for (; blk < n_blocks; blk += stride) {
+  // DW: stage rows, this wavefront's 2 x KW blocks of dW
+  constexpr int SP = 128 * ES + 32, NPAIR = NB / 2, KW = NB == 8 ? 4 : 2;
+  char* stage_z = lds_t + G::t_bytes(DW ? 128 : 0);
+  char* stage_x = stage_z + 128 * SP;
+  const int dw_n = (wave % NPAIR) * 32, dw_k = (wave / NPAIR) * (KW * 16);
+  la_f32x4_t wacc[DW ? 2 : 1][DW ? KW : 1];
+#pragma unroll
+  for (int i = 0; i < (DW ? 2 : 1); ++i)
+#pragma unroll
+    for (int j = 0; j < (DW ? KW : 1); ++j) wacc[i][j] = la_f32x4_t{0.f, 0.f, 0.f, 0.f};
+  if ((DW ? blk - wave : blk) < n_blocks) load_x(blk, 0, xc);
+  for (; (DW ? blk - wave : blk) < n_blocks; blk += stride) {
+    if constexpr (DW) {
+      __syncthreads();                                         // the stage is read
+#pragma unroll
+      for (int s = 0; s < KC; ++s)
+        *reinterpret_cast<uint4*>(stage_x + (wave * 16 + r16) * SP + s * 64 + q * 16) = s < KS ? xc[s] : make_uint4(0u, 0u, 0u, 0u);
+    }
     // the parameters are read from LDS block after block: hoisted out of the loop they would take up to 96 registers
     asm volatile("" ::: "memory");
     const bool row_ok = r16 <= (int)min((int64_t)15, m_rows - 1 - blk * 16);
@@ -243,11 +266,12 @@ __global__ __launch_bounds__(kLsThreads) void linear_stream_kernel(LsArgs a) {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) rv[nb] = typename Raw4<T>::type{};
     if (a.r) {
-      const char* base = reinterpret_cast<const char*>(a.r) + blk * 16 * a.r_ld * ES;
-      const uint32_t off = (uint32_t)lane_row(blk) * (uint32_t)(a.r_ld * ES) + (VEC ? q * 4 * ES : 0);
+      const int64_t b = DW ? min(blk, n_blocks - 1) : blk;
+      const char* base = reinterpret_cast<const char*>(a.r) + b * 16 * a.r_ld * ES;
+      const uint32_t off = (uint32_t)lane_row(b) * (uint32_t)(a.r_ld * ES) + (NV ? q * 4 * ES : 0);
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
-        if constexpr (VEC) {
+        if constexpr (NV) {
           if (n_full || nb * 16 < N) rv[nb] = *reinterpret_cast<const typename Raw4<T>::type*>(base + off + nb * 16 * ES);
         } else {
           rv[nb] = ls_load4<T>(reinterpret_cast<const T*>(base + off), nb * 16 + q * 4, N, 0);
@@ -313,8 +337,8 @@ __global__ __launch_bounds__(kLsThreads) void linear_stream_kernel(LsArgs a) {
         const uint32_t off = (uint32_t)r16 * (uint32_t)(width * sizeof(O)) + q * 4 * sizeof(O);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
-          if ((VEC ? nb * 16 : nb * 16 + q * 4) < N)
-            la_store4<O>(reinterpret_cast<O*>(base + off + nb * 16 * sizeof(O)), VEC ? 4 : N - nb * 16 - q * 4, VEC, val[nb]);
+          if ((NV ? nb * 16 : nb * 16 + q * 4) < N)
+            la_store4<O>(reinterpret_cast<O*>(base + off + nb * 16 * sizeof(O)), NV ? 4 : N - nb * 16 - q * 4, NV, val[nb]);
       };
       // (channel block by channel block: whole-row arrays of intermediates do not fit beside the sums and the next block's x)
       if constexpr (!BWD) {
@@ -394,7 +418,7 @@ __global__ __launch_bounds__(kLsThreads) void linear_stream_kernel(LsArgs a) {
           for (int i = 0; i < NB * 4; ++i) t[i] = d[i / 4][i % 4];
           add_rows(NSUM ? NSUM - 1 : 0, t);
         }
-        if (row_ok) store_rows(reinterpret_cast<T*>(a.out), d, N);
+        if (!DW && row_ok) store_rows(reinterpret_cast<T*>(a.out), d, N);
         if constexpr (DX) {
           // dz as the operand of dz . W: step s of n = this lane's registers 2 s, 2 s + 1 (16-bit, rounded once) or s (f32)
           uint4 f[G::NS];
@@ -409,9 +433,34 @@ __global__ __launch_bounds__(kLsThreads) void linear_stream_kernel(LsArgs a) {
               f[s] = Vec16<T>::pack(t);
             }
           }
+          if constexpr (DW) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+              *reinterpret_cast<uint2*>(stage_z + (wave * 16 + r16) * SP + (nb * 16 + q * 4) * 2) =
+                  nb & 1 ? make_uint2(f[nb / 2].z, f[nb / 2].w) : make_uint2(f[nb / 2].x, f[nb / 2].y);
+            __syncthreads();                                   // the stage is written
+            auto tr = [&](const char* stage, int ms, int col) {
+              const char* p = stage + (ms * 32 + q * 8 + (r16 >> 2)) * SP + col * 2 + (r16 & 3) * 8;
+              const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) la_s4_t*)p));
+              const uint2 hi = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) la_s4_t*)(p + 4 * SP)));
+              return make_uint4(lo.x, lo.y, hi.x, hi.y);
+            };
+#pragma unroll
+            for (int ms = 0; ms < 4; ++ms) {
+              uint4 fz[2];
+#pragma unroll
+              for (int i = 0; i < 2; ++i) fz[i] = tr(stage_z, ms, dw_n + i * 16);
+#pragma unroll
+              for (int j = 0; j < KW; ++j) {
+                const uint4 fx = tr(stage_x, ms, dw_k + j * 16);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) wacc[i][j] = la_mfma<T>(fz[i], fx, wacc[i][j]);
+              }
+            }
+          }
           char* base = reinterpret_cast<char*>(a.gx) + blk * 16 * K * ES;
           const uint32_t off = (uint32_t)r16 * (uint32_t)(K * ES) + q * 4 * ES;
-          const int kb_end = (K + 15) / 16;
+          const int kb_end = DW && !a.gx ? 0 : (K + 15) / 16;
           for (int kg = 0; kg < kb_end; kg += 4) {
             la_f32x4_t o[4];
 #pragma unroll
@@ -428,7 +477,7 @@ __global__ __launch_bounds__(kLsThreads) void linear_stream_kernel(LsArgs a) {
             for (int t = 0; t < 4; ++t) {
               const int k = (kg + t) * 16 + q * 4;
               const float o4[4] = {o[t][0], o[t][1], o[t][2], o[t][3]};
-              if (row_ok && k < K) la_store4<T>(reinterpret_cast<T*>(base + (kg + t) * 16 * ES + off), VEC ? 4 : K - k, VEC, o4);
+              if (row_ok && k < K) la_store4<T>(reinterpret_cast<T*>(base + (kg + t) * 16 * ES + off), NV ? 4 : K - k, NV, o4);
             }
           }
         }
@@ -457,6 +506,18 @@ __global__ __launch_bounds__(kLsThreads) void linear_stream_kernel(LsArgs a) {
       for (int w = 0; w < waves; ++w) t += red[(w * NSUM + s) * NP + n];
       slab[(int64_t)s * N + n] = t;
     }
+    if constexpr (DW) {                                        // behind the sums: this workgroup's dW (n, k)
+      float* dw = slab + (int64_t)NSUM * N;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < KW; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int n = dw_n + i * 16 + q * 4 + e, k = dw_k + j * 16 + r16;
+            if (n < N && k < K) dw[(int64_t)n * K + k] = wacc[i][j][e];
+          }
+    }
   }
 }
 
@@ -464,36 +525,40 @@ __global__ __launch_bounds__(kLsThreads) void linear_stream_kernel(LsArgs a) {
 constexpr int kLsLds = 158 * 1024;                             // a CU has 160 KB
 constexpr int ls_nb(int64_t n) { return n <= 16 ? 1 : n <= 32 ? 2 : n <= 64 ? 4 : n <= 128 ? 8 : n <= 256 ? 16 : 0; }
 
-template <typename T, int NB> static int ls_lds(int k, int sums, bool dx) {
+template <typename T, int NB> static int ls_lds(int k, int sums, bool dx, bool dw = false) {
   using G = LsGeom<T, NB>;
   const int red = std::max(G::w_bytes(k), (kLsThreads / kWave) * sums * G::NP * 4);
-  return red + G::param_bytes + (dx ? G::t_bytes(k) : 0);
+  return red + G::param_bytes + (dx ? G::t_bytes(dw ? 128 : k) : 0) + (dw ? 2 * 128 * (128 * (int)sizeof(T) + 32) : 0);
 }
 // bytes of LDS a launch over (k, n) needs (beyond kLsLds, or n beyond 256: the tiled product takes over)
-template <typename T> static int ls_lds_any(int64_t k, int64_t n, int sums, bool dx) {
+template <typename T> static int ls_lds_any(int64_t k, int64_t n, int sums, bool dx, bool dw = false) {
   if (k > 4096) return INT32_MAX;
   switch (ls_nb(n)) {
-    case 1: return ls_lds<T, 1>((int)k, sums, dx);
-    case 2: return ls_lds<T, 2>((int)k, sums, dx);
-    case 4: return ls_lds<T, 4>((int)k, sums, dx);
-    case 8: return ls_lds<T, 8>((int)k, sums, dx);
-    case 16: return ls_lds<T, 16>((int)k, sums, dx);
+    case 1: return ls_lds<T, 1>((int)k, sums, dx, dw);
+    case 2: return ls_lds<T, 2>((int)k, sums, dx, dw);
+    case 4: return ls_lds<T, 4>((int)k, sums, dx, dw);
+    case 8: return ls_lds<T, 8>((int)k, sums, dx, dw);
+    case 16: return ls_lds<T, 16>((int)k, sums, dx, dw);
   }
   return INT32_MAX;
+}
+// the fused weight gradient: 16-bit rows of up to 128 values on both sides
+template <typename T> static bool ls_dw_fits(int64_t k, int64_t n, int sums) {
+  return sizeof(T) == 2 && k <= 128 && (ls_nb(n) == 4 || ls_nb(n) == 8) && ls_lds_any<T>(k, n, sums, true, true) <= kLsLds;
 }
 
 // channels of a streaming backward pass: beyond 128, xh, dz and the temporaries of the three sums do not fit a lane's 256 registers
 constexpr int ls_bwd_max(int norm) { return norm ? 128 : 256; }
 constexpr int kLsGrid = 512;                                   // workgroups of a launch: two per CU where LDS and registers allow
 
-template <typename T, int NB, int EPI, bool DX, bool VEC> static int ls_go(LsArgs a, int* n_slabs, hipStream_t st) {
+template <typename T, int NB, int EPI, bool DX, int VEC, bool DW = false> static int ls_go(LsArgs a, int* n_slabs, hipStream_t st) {
   constexpr int NSUM = EPI == LS_DNORM ? 3 : EPI == LS_DACT ? 1 : 0;
-  const int lds = ls_lds<T, NB>(a.k, NSUM, DX);
-  a.red_bytes = lds - LsGeom<T, NB>::param_bytes - (DX ? LsGeom<T, NB>::t_bytes(a.k) : 0);
+  const int lds = ls_lds<T, NB>(a.k, NSUM, DX, DW);
+  a.red_bytes = ls_lds<T, NB>(a.k, NSUM, false) - LsGeom<T, NB>::param_bytes;
   static bool attr_set_dev[64] = {};
   bool& attr_set = per_device_flag(attr_set_dev);
   if (!attr_set) {
-    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&linear_stream_kernel<T, NB, EPI, DX, VEC>), hipFuncAttributeMaxDynamicSharedMemorySize, kLsLds);
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&linear_stream_kernel<T, NB, EPI, DX, VEC, DW>), hipFuncAttributeMaxDynamicSharedMemorySize, kLsLds);
     if (e != hipSuccess) { set_error("linear_stream: cannot reserve %d B of LDS: %s", kLsLds, hipGetErrorString(e)); return PYGHO_ERR_LAUNCH; }
     attr_set = true;
   }
@@ -503,13 +568,13 @@ template <typename T, int NB, int EPI, bool DX, bool VEC> static int ls_go(LsArg
   const int threads = NSUM == 0 && blocks < 256 * 8 ? 256 : kLsThreads;
   const int grid = (int)std::min<int64_t>(ceil_div(blocks, threads / kWave), lds <= 80 * 1024 ? kLsGrid : kLsGrid / 2);
   if (n_slabs) *n_slabs = grid;
-  hipLaunchKernelGGL((linear_stream_kernel<T, NB, EPI, DX, VEC>), dim3(grid), dim3(threads), lds, st, a);
+  hipLaunchKernelGGL((linear_stream_kernel<T, NB, EPI, DX, VEC, DW>), dim3(grid), dim3(threads), lds, st, a);
   return check_launch("linear_stream");
 }
 
-// One 16-row block per wavefront and turn: the registers go to the epilogue, the sums and the prefetch, and reading W's fragments costs 16 of
-// the ~85 cycles that HBM takes per row at K = N = 128, 64 of 114 at 256
-template <typename T, int EPI, bool DX, bool VEC> static int ls_pick_vec(const LsArgs& a, int* n_slabs, hipStream_t st) {
+// One 16-row block per wavefront and turn: the registers go to the epilogue and the prefetch; reading W's fragments costs 16 of the ~85 cycles that HBM
+// takes per row at K = N = 128
+template <typename T, int EPI, bool DX, int VEC> static int ls_pick_vec(const LsArgs& a, int* n_slabs, hipStream_t st) {
   switch (ls_nb(a.n)) {
     case 1: return ls_go<T, 1, EPI, DX, VEC>(a, n_slabs, st);
     case 2: return ls_go<T, 2, EPI, DX, VEC>(a, n_slabs, st);
@@ -523,7 +588,16 @@ template <typename T, int EPI, bool DX, bool VEC> static int ls_pick_vec(const L
   return PYGHO_ERR_UNSUPPORTED;
 }
 template <typename T, int EPI, bool DX> static int ls_pick(const LsArgs& a, int* n_slabs, hipStream_t st) {
-  return a.vec ? ls_pick_vec<T, EPI, DX, true>(a, n_slabs, st) : ls_pick_vec<T, EPI, DX, false>(a, n_slabs, st);
+  if (a.vec == 3) return ls_pick_vec<T, EPI, DX, 3>(a, n_slabs, st);
+  return a.vec & 1 ? ls_pick_vec<T, EPI, DX, 1>(a, n_slabs, st) : ls_pick_vec<T, EPI, DX, 0>(a, n_slabs, st);
+}
+template <typename T, int EPI> static int ls_pick_dw(const LsArgs& a, int* n_slabs, hipStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    if (ls_nb(a.n) == 4) return ls_go<T, 4, EPI, true, 3, true>(a, n_slabs, st);
+    if (ls_nb(a.n) == 8) return ls_go<T, 8, EPI, true, 3, true>(a, n_slabs, st);
+  }
+  set_error("linear_stream: no fused weight gradient for %d channels", a.n);
+  return PYGHO_ERR_UNSUPPORTED;
 }
 
 }  // namespace pygho
