@@ -9,13 +9,15 @@
 
 namespace pygho {
 
+constexpr int kLoThreads = 512;
+
 // 16-row blocks of a wavefront and turn: two, one for the longest f32 rows (their x and the next block's would not fit beside the products, and an f32
 // fragment already feeds four MFMAs of 32 cycles)
 template <typename T, int KS> constexpr int lo_blocks() { return sizeof(T) == 4 && KS == 8 ? 1 : 2; }
 
 // KS: 64-byte steps of k held in registers
 template <typename T, int KS, int VEC>
-__global__ __launch_bounds__(kLsThreads) void linear_out_kernel(LsArgs a) {
+__global__ __launch_bounds__(kLoThreads) void linear_out_kernel(LsArgs a) {
   constexpr bool P = Precise<T>::value;
   constexpr bool XV = VEC & 1, NV = VEC & 2;                   // as in linear_stream.h
   constexpr int ES = sizeof(T), E = 16 / ES, MB = lo_blocks<T, KS>(), PITCH = KS * 64 + 16;
@@ -146,8 +148,8 @@ template <typename T, int KS, int VEC> static int lo_go(const LsArgs& a, hipStre
   }
   const int lds = lo_lds<T>(a.k, a.n);
   const int64_t blocks = ceil_div(a.m, 16 * lo_blocks<T, KS>());
-  const int threads = blocks < 256 * 8 ? 256 : kLsThreads;
-  const int grid = (int)std::min<int64_t>(ceil_div(blocks, threads / kWave), lds <= 80 * 1024 ? kLsGrid : kLsGrid / 2);
+  const int threads = blocks < 256 * 8 ? 256 : kLoThreads;
+  const int grid = (int)std::min<int64_t>(ceil_div(blocks, threads / kWave), lds <= 80 * 1024 ? 512 : 256);
   hipLaunchKernelGGL((linear_out_kernel<T, KS, VEC>), dim3(grid), dim3(threads), lds, st, a);
   return check_launch("linear_out");
 }

@@ -7,7 +7,7 @@
 //   * swapped MFMA (D[n][m]): a lane ends up with 4 consecutive channels of ONE row, a row's channels sit in 4 lanes: bias (the accumulator's
 //     start value), norm, activation, residual and the store happen in those registers;
 //   * backward: dz leaves the epilogue in exactly the lanes and order in which the product dz . W wants its operand (the order of n inside
-//     a reduction is free as long as W's copy has the same one), so dX follows in the same launch without moving a value;
+//     a reduction is free as long as W is read in the same one), so dX follows in the same launch without moving a value;
 //   * channel sums (gg, gh, gb) are taken from the unrounded f32 values, over a block's 16 rows by lane exchanges (ls_row_sums).
 // Block b of the rows belongs to wavefront b % (all wavefronts), so sums depend on the true row count only (see layer_norm.hip).
 #pragma once
@@ -84,6 +84,13 @@ template <typename T> __device__ __forceinline__ void ls_unpack4(const typename 
   }
 }
 
+// 8 16-bit values per lane out of a row-major LDS tile, transposed: lane r16 gets column r16 of 4 rows at p's 16 lanes and of 4 rows `dist` bytes on
+__device__ __forceinline__ uint4 ls_read_tr(const char* p, int dist) {
+  const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) la_s4_t*)p));
+  const uint2 hi = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) la_s4_t*)(p + dist)));
+  return make_uint4(lo.x, lo.y, hi.x, hi.y);
+}
+
 // Sums over the 16 rows of a block (lanes r16 of a group): V values per lane -> their totals dealt out over the lanes.  A step gives half of the values
 // to the partner lane and takes the partner's half of the others: V / 2 additions instead of V.  Partners i ^ 15, ^ 7, ^ 3, ^ 1 are single DPP
 // moves; `up[s]` says which half a lane keeps (bit 3 - s of its number).  Lane i ends up with values [i * V / 16, + V / 16); below 16 values the
@@ -106,37 +113,36 @@ template <int V, int S> __device__ __forceinline__ void ls_row_sums(float (&v)[V
   }
 }
 
-// position of reduction index n in the transposed copy of W: the order in which a lane's accumulators hold it.  16-bit: a step is 32 n, lane
-// group q holds 4 q .. 4 q + 3 of its first and of its second 16; f32: a step is 16 n, lane group q holds 4 q .. 4 q + 3
-template <typename T> __device__ __forceinline__ int ls_perm(int n) {
-  if constexpr (sizeof(T) == 4) return n;
-  return (n & ~31) | (((n >> 2) & 3) << 3) | (((n >> 4) & 1) << 2) | (n & 3);
-}
-
-constexpr int kLsThreads = 512;
+// wavefronts per SIMD the registers are limited to (512 / this many per lane): latency, not throughput, is what a turn of 16 rows has most of
+// (element-wise accesses beside the gradient through a norm of 65 .. 128 channels: 168 registers do not hold them)
+constexpr int ls_wps(int nb, int epi, int vec) { return nb <= 4 ? 4 : nb <= 8 && !(epi == LS_DNORM && vec != 3) ? 3 : 2; }
 
 // geometry that host and device share
 template <typename T, int NB> struct LsGeom {
   static constexpr int ES = sizeof(T), NP = NB * 16;
   static constexpr int NS = (NP * ES + 63) / 64;               // 64-byte steps over n (dX)
-  static constexpr int PITCH_T = NS * 64 + 16;                 // a row of the transposed copy
+  static constexpr int ROWS = NS * 64 / ES;                    // rows of W in LDS: whole steps of n (zeros beyond NP)
+  static constexpr int PITCH_T = NS * 64 + 16;                 // f32: a row of the copy with n contiguous
   __host__ __device__ static int steps(int k) { return (k * ES + 63) / 64; }
   __host__ __device__ static int pitch_w(int k) { return steps(k) * 64 + 16; }
   __host__ __device__ static int rows_t(int k) { return (k + 15) / 16 * 16; }
-  __host__ __device__ static int w_bytes(int k) { return NP * pitch_w(k); }
-  __host__ __device__ static int t_bytes(int k) { return rows_t(k) * PITCH_T; }
+  __host__ __device__ static int w_bytes(int k) { return ROWS * pitch_w(k); }
+  // 16-bit: dX reads W transposed (ds_read_b64_tr_b16); f32 has no such read and keeps the copy
+  __host__ __device__ static int t_bytes(int k) { return ES == 2 ? 0 : rows_t(k) * PITCH_T; }
   static constexpr int param_bytes = 4 * NP * 4;
 };
+// the fused weight gradient: workgroups of 4 wavefronts, two per CU, each at its own place in the sequence of phases between its barriers
+constexpr int kLsDwWaves = 4;
 
 // VEC & 1: k is a whole number of 64-byte steps and x's rows allow 16-byte accesses.  VEC & 2: n is a whole number of 16 channels and the rows of r, out
 // and gx allow accesses of 4 elements (k of 16, with gx).  A block's rows then are one uniform base address, one 32-bit offset per lane and
 // constants -- 64-bit addresses per access, or masks per element, take more registers than the sums do.  Otherwise element by element.
 //
-// DW (16-bit, k <= 128): the weight gradient in the same launch.  The workgroup's 8 wavefronts go through their blocks in step; each puts its dz
-// and its x (16 rows, row-major) into LDS, and after a barrier forms its share of dW += dz^T x over the 128 rows, both operands read back
+// DW (16-bit, k <= 128): the weight gradient in the same launch.  The workgroup's wavefronts go through their blocks in step; each puts its dz
+// and its x (16 rows, row-major) into LDS, and after a barrier forms its share of dW += dz^T x over the 64 rows, both operands read back
 // transposed by the LDS (ds_read_b64_tr_b16).  dz never reaches memory and x is read once: 3 streams instead of 6
 template <typename T, int NB, int EPI, bool DX, int VEC, bool DW = false>
-__global__ __launch_bounds__(kLsThreads) void linear_stream_kernel(LsArgs a) {
+__global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC) * 256, DW ? 2 : ls_wps(NB, EPI, VEC)) void linear_stream_kernel(LsArgs a) {
   using G = LsGeom<T, NB>;
   constexpr bool P = Precise<T>::value, BWD = EPI == LS_DACT || EPI == LS_DNORM, NORM = EPI == LS_NORM || EPI == LS_DNORM;
   constexpr int ES = G::ES, E = 16 / ES, NP = G::NP, KC = 4;
@@ -157,7 +163,7 @@ __global__ __launch_bounds__(kLsThreads) void linear_stream_kernel(LsArgs a) {
   // ---- W -> LDS (padding: zeros) ----------------------------------------------------------------------------------------------------
   if (!a.w_trans) {
     const int cpr = KS * 4;                                    // 16-byte chunks per row
-    for (int c = threadIdx.x; c < NP * cpr; c += blockDim.x) {
+    for (int c = threadIdx.x; c < G::ROWS * cpr; c += blockDim.x) {
       const int n = c / cpr, kc = c - n * cpr;
       uint4 v = make_uint4(0u, 0u, 0u, 0u);
       if (n < N) v = ls_load16<T>(wp + (int64_t)n * a.w_ld, kc * E, K, a.w_vec);
@@ -178,20 +184,15 @@ __global__ __launch_bounds__(kLsThreads) void linear_stream_kernel(LsArgs a) {
       }
     }
   }
-  if constexpr (DX) {                                          // the copy with n contiguous: rows k, columns ls_perm(n)
-    const int kr = G::rows_t(K), ck = (kr + E - 1) / E, np = G::NS * 64 / ES;
-    for (int c = threadIdx.x; c < np * ck; c += blockDim.x) {
-      const int n = c / ck, kc = c - n * ck, pn = ls_perm<T>(n);
-      union { uint4 u; uint16_t h[8]; uint32_t f[4]; } v;
+  if constexpr (DX && ES == 4) {                               // the copy with n contiguous
+    const int kr = G::rows_t(K), ck = kr / E;
+    for (int c = threadIdx.x; c < G::ROWS * ck; c += blockDim.x) {
+      const int n = c / ck, kc = c - n * ck;
+      union { uint4 u; uint32_t f[4]; } v;
       v.u = make_uint4(0u, 0u, 0u, 0u);
       if (n < N) v.u = ls_load16<T>(wp + (int64_t)n * a.w_ld, kc * E, K, a.w_vec);
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const int k = kc * E + j;
-        if (k >= kr) break;
-        if constexpr (ES == 2) *reinterpret_cast<uint16_t*>(lds_t + k * G::PITCH_T + pn * 2) = v.h[j];
-        else *reinterpret_cast<uint32_t*>(lds_t + k * G::PITCH_T + pn * 4) = v.f[j];
-      }
+      for (int j = 0; j < E; ++j) *reinterpret_cast<uint32_t*>(lds_t + (kc * E + j) * G::PITCH_T + n * 4) = v.f[j];
     }
   }
   for (int n = threadIdx.x; n < NP; n += blockDim.x) {
@@ -240,16 +241,16 @@ __global__ __launch_bounds__(kLsThreads) void linear_stream_kernel(LsArgs a) {
     }
   };
   int64_t blk = (int64_t)blockIdx.x * waves + wave;
-  // DW: stage rows, this wavefront's 2 x KW blocks of dW
-  constexpr int SP = 128 * ES + 32, NPAIR = NB / 2, KW = NB == 8 ? 4 : 2;
-  char* stage_z = lds_t + G::t_bytes(DW ? 128 : 0);
-  char* stage_x = stage_z + 128 * SP;
-  const int dw_n = (wave % NPAIR) * 32, dw_k = (wave / NPAIR) * (KW * 16);
-  la_f32x4_t wacc[DW ? 2 : 1][DW ? KW : 1];
+  // DW: stage rows, this wavefront's NW x KW blocks of dW
+  constexpr int SP = 128 * ES + 32, SR = kLsDwWaves * 16, NW = DW ? NB / 2 : 1, KW = DW ? 4 : 1;
+  char* stage_z = lds_t;
+  char* stage_x = stage_z + SR * SP;
+  const int dw_n = (wave & 1) * (NW * 16), dw_k = (wave >> 1) * (KW * 16);
+  la_f32x4_t wacc[NW][KW];
 #pragma unroll
-  for (int i = 0; i < (DW ? 2 : 1); ++i)
+  for (int i = 0; i < NW; ++i)
 #pragma unroll
-    for (int j = 0; j < (DW ? KW : 1); ++j) wacc[i][j] = la_f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < KW; ++j) wacc[i][j] = la_f32x4_t{0.f, 0.f, 0.f, 0.f};
   if ((DW ? blk - wave : blk) < n_blocks) load_x(blk, 0, xc);
   for (; (DW ? blk - wave : blk) < n_blocks; blk += stride) {
     if constexpr (DW) {
@@ -260,6 +261,8 @@ __global__ __launch_bounds__(kLsThreads) void linear_stream_kernel(LsArgs a) {
     }
     // the parameters are read from LDS block after block: hoisted out of the loop they would take up to 96 registers
     asm volatile("" ::: "memory");
+    int N_here = N;                                            // (likewise: the comparisons with n, not 16 masks kept for the whole loop)
+    asm volatile("" : "+s"(N_here));
     const bool row_ok = r16 <= (int)min((int64_t)15, m_rows - 1 - blk * 16);
     // the residual's / the output gradient's 4 channels per lane and 16: in flight during the products
     typename Raw4<T>::type rv[NB];
@@ -272,10 +275,18 @@ __global__ __launch_bounds__(kLsThreads) void linear_stream_kernel(LsArgs a) {
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         if constexpr (NV) {
-          if (n_full || nb * 16 < N) rv[nb] = *reinterpret_cast<const typename Raw4<T>::type*>(base + off + nb * 16 * ES);
+          if (nb * 16 < N_here) rv[nb] = *reinterpret_cast<const typename Raw4<T>::type*>(base + off + nb * 16 * ES);
         } else {
           rv[nb] = ls_load4<T>(reinterpret_cast<const T*>(base + off), nb * 16 + q * 4, N, 0);
         }
+      }
+    }
+    if (BWD && (blk + 1) * 16 > m_rows) {                      // a repeated row adds nothing to the sums: its gradient is zero
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        rv[nb].x = row_ok ? rv[nb].x : 0u;
+        rv[nb].y = row_ok ? rv[nb].y : 0u;
+        if constexpr (ES == 4) { rv[nb].z = row_ok ? rv[nb].z : 0u; rv[nb].w = row_ok ? rv[nb].w : 0u; }
       }
     }
     la_f32x4_t acc[NB];
@@ -337,7 +348,7 @@ __global__ __launch_bounds__(kLsThreads) void linear_stream_kernel(LsArgs a) {
         const uint32_t off = (uint32_t)r16 * (uint32_t)(width * sizeof(O)) + q * 4 * sizeof(O);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
-          if ((NV ? nb * 16 : nb * 16 + q * 4) < N)
+          if ((NV ? nb * 16 : nb * 16 + q * 4) < N_here)
             la_store4<O>(reinterpret_cast<O*>(base + off + nb * 16 * sizeof(O)), NV ? 4 : N - nb * 16 - q * 4, NV, val[nb]);
       };
       // (channel block by channel block: whole-row arrays of intermediates do not fit beside the sums and the next block's x)
@@ -366,8 +377,6 @@ __global__ __launch_bounds__(kLsThreads) void linear_stream_kernel(LsArgs a) {
         for (int nb = 0; nb < NB; ++nb) {
           const int n = nb * 16 + q * 4;
           ls_unpack4<T>(rv[nb], d[nb]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) d[nb][e] = row_ok ? d[nb][e] : 0.f;      // a repeated row adds nothing to the sums
           if constexpr (NORM) {
             const float4 g4 = *reinterpret_cast<const float4*>(lds_g + n);
             const float gv[4] = {g4.x, g4.y, g4.z, g4.w};
@@ -440,41 +449,41 @@ __global__ __launch_bounds__(kLsThreads) void linear_stream_kernel(LsArgs a) {
                   nb & 1 ? make_uint2(f[nb / 2].z, f[nb / 2].w) : make_uint2(f[nb / 2].x, f[nb / 2].y);
             __syncthreads();                                   // the stage is written
             auto tr = [&](const char* stage, int ms, int col) {
-              const char* p = stage + (ms * 32 + q * 8 + (r16 >> 2)) * SP + col * 2 + (r16 & 3) * 8;
-              const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) la_s4_t*)p));
-              const uint2 hi = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) la_s4_t*)(p + 4 * SP)));
-              return make_uint4(lo.x, lo.y, hi.x, hi.y);
+              return ls_read_tr(stage + (ms * 32 + q * 8 + (r16 >> 2)) * SP + col * 2 + (r16 & 3) * 8, 4 * SP);
             };
 #pragma unroll
-            for (int ms = 0; ms < 4; ++ms) {
-              uint4 fz[2];
+            for (int ms = 0; ms < SR / 32; ++ms) {
+              uint4 fz[NW];
 #pragma unroll
-              for (int i = 0; i < 2; ++i) fz[i] = tr(stage_z, ms, dw_n + i * 16);
+              for (int i = 0; i < NW; ++i) fz[i] = tr(stage_z, ms, dw_n + i * 16);
 #pragma unroll
               for (int j = 0; j < KW; ++j) {
                 const uint4 fx = tr(stage_x, ms, dw_k + j * 16);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) wacc[i][j] = la_mfma<T>(fz[i], fx, wacc[i][j]);
+                for (int i = 0; i < NW; ++i) wacc[i][j] = la_mfma<T>(fz[i], fx, wacc[i][j]);
               }
             }
           }
           char* base = reinterpret_cast<char*>(a.gx) + blk * 16 * K * ES;
           const uint32_t off = (uint32_t)r16 * (uint32_t)(K * ES) + q * 4 * ES;
           const int kb_end = DW && !a.gx ? 0 : (K + 15) / 16;
-          for (int kg = 0; kg < kb_end; kg += 4) {
-            la_f32x4_t o[4];
+          constexpr int KG = NORM ? 2 : 4;                     // 16-channel blocks at once (the norm's registers leave room for two)
+          for (int kg = 0; kg < kb_end; kg += KG) {
+            la_f32x4_t o[KG];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) o[t] = la_f32x4_t{0.f, 0.f, 0.f, 0.f};
+            for (int t = 0; t < KG; ++t) o[t] = la_f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int s = 0; s < G::NS; ++s)
 #pragma unroll
-              for (int t = 0; t < 4; ++t) {
+              for (int t = 0; t < KG; ++t) {
                 const int kb = min(kg + t, kb_end - 1);        // (a block past the end is formed again and not stored)
-                const uint4 fa = *reinterpret_cast<const uint4*>(lds_t + (kb * 16 + r16) * G::PITCH_T + s * 64 + q * 16);
+                uint4 fa;                                      // row k, and n in the order of f[s]
+                if constexpr (ES == 4) fa = *reinterpret_cast<const uint4*>(lds_t + (kb * 16 + r16) * G::PITCH_T + s * 64 + q * 16);
+                else fa = ls_read_tr(lds_w + (s * 32 + q * 4 + (r16 >> 2)) * pitch + kb * 32 + (r16 & 3) * 8, 16 * pitch);
                 o[t] = la_mfma<T>(fa, f[s], o[t]);
               }
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
+            for (int t = 0; t < KG; ++t) {
               const int k = (kg + t) * 16 + q * 4;
               const float o4[4] = {o[t][0], o[t][1], o[t][2], o[t][3]};
               if (row_ok && k < K) la_store4<T>(reinterpret_cast<T*>(base + (kg + t) * 16 * ES + off), NV ? 4 : K - k, NV, o4);
@@ -509,7 +518,7 @@ __global__ __launch_bounds__(kLsThreads) void linear_stream_kernel(LsArgs a) {
     if constexpr (DW) {                                        // behind the sums: this workgroup's dW (n, k)
       float* dw = slab + (int64_t)NSUM * N;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < NW; ++i)
 #pragma unroll
         for (int j = 0; j < KW; ++j)
 #pragma unroll
@@ -522,13 +531,16 @@ __global__ __launch_bounds__(kLsThreads) void linear_stream_kernel(LsArgs a) {
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------------------
-constexpr int kLsLds = 158 * 1024;                             // a CU has 160 KB
+constexpr int kLsLds = 158 * 1024;                             // a workgroup's share of the CU's 160 KB
 constexpr int ls_nb(int64_t n) { return n <= 16 ? 1 : n <= 32 ? 2 : n <= 64 ? 4 : n <= 128 ? 8 : n <= 256 ? 16 : 0; }
 
+template <typename T, int NB> static int ls_red(int k, int sums) {      // W, and at the end the wavefronts' sums in its place
+  using G = LsGeom<T, NB>;
+  return std::max(G::w_bytes(k), ls_wps(NB, LS_ACT, 3) * 4 * sums * G::NP * 4);
+}
 template <typename T, int NB> static int ls_lds(int k, int sums, bool dx, bool dw = false) {
   using G = LsGeom<T, NB>;
-  const int red = std::max(G::w_bytes(k), (kLsThreads / kWave) * sums * G::NP * 4);
-  return red + G::param_bytes + (dx ? G::t_bytes(dw ? 128 : k) : 0) + (dw ? 2 * 128 * (128 * (int)sizeof(T) + 32) : 0);
+  return ls_red<T, NB>(k, sums) + G::param_bytes + (dx ? G::t_bytes(k) : 0) + (dw ? 2 * kLsDwWaves * 16 * (128 * (int)sizeof(T) + 32) : 0);
 }
 // bytes of LDS a launch over (k, n) needs (beyond kLsLds, or n beyond 256: the tiled product takes over)
 template <typename T> static int ls_lds_any(int64_t k, int64_t n, int sums, bool dx, bool dw = false) {
@@ -544,17 +556,17 @@ template <typename T> static int ls_lds_any(int64_t k, int64_t n, int sums, bool
 }
 // the fused weight gradient: 16-bit rows of up to 128 values on both sides
 template <typename T> static bool ls_dw_fits(int64_t k, int64_t n, int sums) {
-  return sizeof(T) == 2 && k <= 128 && (ls_nb(n) == 4 || ls_nb(n) == 8) && ls_lds_any<T>(k, n, sums, true, true) <= kLsLds;
+  return sizeof(T) == 2 && k <= 128 && (ls_nb(n) == 4 || ls_nb(n) == 8) && ls_lds_any<T>(k, n, sums, true, true) <= kLsLds / 2;
 }
 
 // channels of a streaming backward pass: beyond 128, xh, dz and the temporaries of the three sums do not fit a lane's 256 registers
 constexpr int ls_bwd_max(int norm) { return norm ? 128 : 256; }
-constexpr int kLsGrid = 512;                                   // workgroups of a launch: two per CU where LDS and registers allow
+constexpr int kLsGrid = 1024;                                  // most workgroups of a launch (and slabs)
 
 template <typename T, int NB, int EPI, bool DX, int VEC, bool DW = false> static int ls_go(LsArgs a, int* n_slabs, hipStream_t st) {
-  constexpr int NSUM = EPI == LS_DNORM ? 3 : EPI == LS_DACT ? 1 : 0;
+  constexpr int NSUM = EPI == LS_DNORM ? 3 : EPI == LS_DACT ? 1 : 0, WPS = ls_wps(NB, EPI, VEC);
   const int lds = ls_lds<T, NB>(a.k, NSUM, DX, DW);
-  a.red_bytes = ls_lds<T, NB>(a.k, NSUM, false) - LsGeom<T, NB>::param_bytes;
+  a.red_bytes = ls_red<T, NB>(a.k, NSUM);
   static bool attr_set_dev[64] = {};
   bool& attr_set = per_device_flag(attr_set_dev);
   if (!attr_set) {
@@ -562,13 +574,17 @@ template <typename T, int NB, int EPI, bool DX, int VEC, bool DW = false> static
     if (e != hipSuccess) { set_error("linear_stream: cannot reserve %d B of LDS: %s", kLsLds, hipGetErrorString(e)); return PYGHO_ERR_LAUNCH; }
     attr_set = true;
   }
-  // few rows: workgroups of 4 wavefronts, so that more CUs take part (a backward launch keeps 8: its sums must not depend on the row count's
-  // upper bound)
+  // workgroups per CU: as many as LDS allows copies of W, the CU's 4 WPS wavefronts divided evenly among them.  With few rows, workgroups of 4
+  // wavefronts, so that more CUs take part (not in a backward: its sums must not depend on the row count's upper bound)
   const int64_t blocks = ceil_div(a.m, 16);
-  const int threads = NSUM == 0 && blocks < 256 * 8 ? 256 : kLsThreads;
-  const int grid = (int)std::min<int64_t>(ceil_div(blocks, threads / kWave), lds <= 80 * 1024 ? kLsGrid : kLsGrid / 2);
+  int per_cu = std::min(WPS, std::max(1, 160 * 1024 / lds));
+  while (WPS * 4 % per_cu != 0) --per_cu;
+  int waves = WPS * 4 / per_cu;
+  if (DW) { waves = kLsDwWaves; per_cu = 2; }
+  else if (NSUM == 0 && blocks < 256 * 4 * WPS) waves = std::min(waves, 4);
+  const int grid = (int)std::min<int64_t>(ceil_div(blocks, waves), 256 * per_cu);
   if (n_slabs) *n_slabs = grid;
-  hipLaunchKernelGGL((linear_stream_kernel<T, NB, EPI, DX, VEC, DW>), dim3(grid), dim3(threads), lds, st, a);
+  hipLaunchKernelGGL((linear_stream_kernel<T, NB, EPI, DX, VEC, DW>), dim3(grid), dim3(waves * kWave), lds, st, a);
   return check_launch("linear_stream");
 }
 

@@ -47,7 +47,7 @@ template <bool P, int N> __device__ __forceinline__ void ro_act_slope(float (&g)
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const float s = ro_sigmoid<P>(z[i]);
-      g[i] *= s * (1.f + z[i] * (1.f - s));
+      g[i] *= fmaf(z[i] * s, 1.f - s, s);                              // s (1 + z (1 - s))
     }
   } else if (act == kActRelu) {
 #pragma unroll
