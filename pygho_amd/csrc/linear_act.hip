@@ -105,7 +105,7 @@ static LaSpace la_space(int64_t m, int64_t k, int64_t n, int norm, int act, int 
     return s;
   }
   s.own_dz = norm || act != kActNone;
-  s.stream = s.own_dz && n <= ls_bwd_max(norm) && la_type(dtype, [&](auto ops) { return ops.stream_lds(k, n, s.nsum, false, false) <= kLsLds; });
+  s.stream = s.own_dz && n <= ls_bwd_max(norm, la_size(dtype)) && la_type(dtype, [&](auto ops) { return ops.stream_lds(k, n, s.nsum, false, false) <= kLsLds; });
   s.dz = s.own_dz ? (m * n * la_size(dtype) + 15) / 16 * 16 : 0;
   s.z = s.own_dz && !s.stream && la_form(k, n, norm, dtype) != FORM_TILE ? (m * n * 4 + 15) / 16 * 16 : 0;
   s.sums = !s.own_dz ? 0 : s.stream ? kLsGrid * la_pad4(s.nsum * n) * 4 : ln_bwd_slab_floats(m, n, s.nsum) * 4;

@@ -114,8 +114,8 @@ template <int V, int S> __device__ __forceinline__ void ls_row_sums(float (&v)[V
 }
 
 // wavefronts per SIMD the registers are limited to (512 / this many per lane): latency, not throughput, is what a turn of 16 rows has most of
-// (element-wise accesses beside the gradient through a norm of 65 .. 128 channels: 168 registers do not hold them)
-constexpr int ls_wps(int nb, int epi, int vec) { return nb <= 4 ? 4 : nb <= 8 && !(epi == LS_DNORM && vec != 3) ? 3 : 2; }
+// (the gradient through a norm of 65 .. 128 channels with the next block's rows in flight: 168 registers do not hold it)
+constexpr int ls_wps(int nb, int epi, int es) { return nb <= 4 ? (nb == 4 && es == 4 && epi == LS_DNORM ? 3 : 4) : nb <= 8 && epi != LS_DNORM ? 3 : 2; }
 
 // geometry that host and device share
 template <typename T, int NB> struct LsGeom {
@@ -142,7 +142,7 @@ constexpr int kLsDwWaves = 4;
 // and its x (16 rows, row-major) into LDS, and after a barrier forms its share of dW += dz^T x over the 64 rows, both operands read back
 // transposed by the LDS (ds_read_b64_tr_b16).  dz never reaches memory and x is read once: 3 streams instead of 6
 template <typename T, int NB, int EPI, bool DX, int VEC, bool DW = false>
-__global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC) * 256, DW ? 2 : ls_wps(NB, EPI, VEC)) void linear_stream_kernel(LsArgs a) {
+__global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, sizeof(T)) * 256, DW ? 2 : ls_wps(NB, EPI, sizeof(T))) void linear_stream_kernel(LsArgs a) {
   using G = LsGeom<T, NB>;
   constexpr bool P = Precise<T>::value, BWD = EPI == LS_DACT || EPI == LS_DNORM, NORM = EPI == LS_NORM || EPI == LS_DNORM;
   constexpr int ES = G::ES, E = 16 / ES, NP = G::NP, KC = 4;
@@ -251,7 +251,32 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC) * 25
   for (int i = 0; i < NW; ++i)
 #pragma unroll
     for (int j = 0; j < KW; ++j) wacc[i][j] = la_f32x4_t{0.f, 0.f, 0.f, 0.f};
-  if ((DW ? blk - wave : blk) < n_blocks) load_x(blk, 0, xc);
+  // the residual's / the output gradient's 4 channels per lane and 16.  They arrive a whole turn ahead: the next block's are asked for as soon as this
+  // block's are used (requested at the top of their own turn they held every wavefront up for most of HBM's latency)
+  typename Raw4<T>::type rv[NB];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) rv[nb] = typename Raw4<T>::type{};
+  constexpr bool AHEAD = !(ES == 4 && NB == 16);               // (256 f32 channels: 64 registers more than there are)
+  auto load_r = [&](int64_t b) {
+    if (!a.r) return;
+    b = min(b, n_blocks - 1);
+    const char* base = reinterpret_cast<const char*>(a.r) + b * 16 * a.r_ld * ES;
+    const uint32_t off = (uint32_t)lane_row(b) * (uint32_t)(a.r_ld * ES) + (NV ? q * 4 * ES : 0);
+    int N_here = N;                                            // (compared here, not held as 16 masks for the whole loop)
+    asm volatile("" : "+s"(N_here));
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      if constexpr (NV) {
+        if (nb * 16 < N_here) rv[nb] = *reinterpret_cast<const typename Raw4<T>::type*>(base + off + nb * 16 * ES);
+      } else {
+        rv[nb] = ls_load4<T>(reinterpret_cast<const T*>(base + off), nb * 16 + q * 4, N, 0);
+      }
+    }
+  };
+  if ((DW ? blk - wave : blk) < n_blocks) {
+    load_x(blk, 0, xc);
+    if constexpr (AHEAD) load_r(blk);
+  }
   for (; (DW ? blk - wave : blk) < n_blocks; blk += stride) {
     if constexpr (DW) {
       __syncthreads();                                         // the stage is read
@@ -261,26 +286,10 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC) * 25
     }
     // the parameters are read from LDS block after block: hoisted out of the loop they would take up to 96 registers
     asm volatile("" ::: "memory");
-    int N_here = N;                                            // (likewise: the comparisons with n, not 16 masks kept for the whole loop)
+    int N_here = N;
     asm volatile("" : "+s"(N_here));
     const bool row_ok = r16 <= (int)min((int64_t)15, m_rows - 1 - blk * 16);
-    // the residual's / the output gradient's 4 channels per lane and 16: in flight during the products
-    typename Raw4<T>::type rv[NB];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) rv[nb] = typename Raw4<T>::type{};
-    if (a.r) {
-      const int64_t b = DW ? min(blk, n_blocks - 1) : blk;
-      const char* base = reinterpret_cast<const char*>(a.r) + b * 16 * a.r_ld * ES;
-      const uint32_t off = (uint32_t)lane_row(b) * (uint32_t)(a.r_ld * ES) + (NV ? q * 4 * ES : 0);
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        if constexpr (NV) {
-          if (nb * 16 < N_here) rv[nb] = *reinterpret_cast<const typename Raw4<T>::type*>(base + off + nb * 16 * ES);
-        } else {
-          rv[nb] = ls_load4<T>(reinterpret_cast<const T*>(base + off), nb * 16 + q * 4, N, 0);
-        }
-      }
-    }
+    if constexpr (!AHEAD) load_r(blk);
     if (BWD && (blk + 1) * 16 > m_rows) {                      // a repeated row adds nothing to the sums: its gradient is zero
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
@@ -367,6 +376,7 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC) * 25
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[nb][e] += r4[e];
         }
+        if constexpr (AHEAD) load_r(blk + stride);
         if (row_ok) {
           if (EPI == LS_ACT && a.out_f32) store_rows(reinterpret_cast<float*>(a.out), v, N);
           else store_rows(reinterpret_cast<T*>(a.out), v, N);
@@ -428,6 +438,7 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC) * 25
           add_rows(NSUM ? NSUM - 1 : 0, t);
         }
         if (!DW && row_ok) store_rows(reinterpret_cast<T*>(a.out), d, N);
+        if constexpr (!DX && AHEAD) load_r(blk + stride);
         if constexpr (DX) {
           // dz as the operand of dz . W: step s of n = this lane's registers 2 s, 2 s + 1 (16-bit, rounded once) or s (f32)
           uint4 f[G::NS];
@@ -442,6 +453,7 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC) * 25
               f[s] = Vec16<T>::pack(t);
             }
           }
+          if constexpr (AHEAD) load_r(blk + stride);                                // (xh and dz have left their registers)
           if constexpr (DW) {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
@@ -536,7 +548,7 @@ constexpr int ls_nb(int64_t n) { return n <= 16 ? 1 : n <= 32 ? 2 : n <= 64 ? 4 
 
 template <typename T, int NB> static int ls_red(int k, int sums) {      // W, and at the end the wavefronts' sums in its place
   using G = LsGeom<T, NB>;
-  return std::max(G::w_bytes(k), ls_wps(NB, LS_ACT, 3) * 4 * sums * G::NP * 4);
+  return std::max(G::w_bytes(k), ls_wps(NB, LS_ACT, sizeof(T)) * 4 * sums * G::NP * 4);
 }
 template <typename T, int NB> static int ls_lds(int k, int sums, bool dx, bool dw = false) {
   using G = LsGeom<T, NB>;
@@ -559,12 +571,12 @@ template <typename T> static bool ls_dw_fits(int64_t k, int64_t n, int sums) {
   return sizeof(T) == 2 && k <= 128 && (ls_nb(n) == 4 || ls_nb(n) == 8) && ls_lds_any<T>(k, n, sums, true, true) <= kLsLds / 2;
 }
 
-// channels of a streaming backward pass: beyond 128, xh, dz and the temporaries of the three sums do not fit a lane's 256 registers
-constexpr int ls_bwd_max(int norm) { return norm ? 128 : 256; }
+// channels of a streaming backward pass: beyond 128, xh, dz and the temporaries of the sums (f32: the rows themselves) do not fit a lane's registers
+constexpr int ls_bwd_max(int norm, int elem_size) { return norm || elem_size == 4 ? 128 : 256; }
 constexpr int kLsGrid = 1024;                                  // most workgroups of a launch (and slabs)
 
 template <typename T, int NB, int EPI, bool DX, int VEC, bool DW = false> static int ls_go(LsArgs a, int* n_slabs, hipStream_t st) {
-  constexpr int NSUM = EPI == LS_DNORM ? 3 : EPI == LS_DACT ? 1 : 0, WPS = ls_wps(NB, EPI, VEC);
+  constexpr int NSUM = EPI == LS_DNORM ? 3 : EPI == LS_DACT ? 1 : 0, WPS = ls_wps(NB, EPI, sizeof(T));
   const int lds = ls_lds<T, NB>(a.k, NSUM, DX, DW);
   a.red_bytes = ls_red<T, NB>(a.k, NSUM);
   static bool attr_set_dev[64] = {};
@@ -597,7 +609,7 @@ template <typename T, int EPI, bool DX, int VEC> static int ls_pick_vec(const Ls
     case 4: return ls_go<T, 4, EPI, DX, VEC>(a, n_slabs, st);
     case 8: return ls_go<T, 8, EPI, DX, VEC>(a, n_slabs, st);
     case 16:
-      if constexpr (EPI != LS_DNORM) return ls_go<T, 16, EPI, DX, VEC>(a, n_slabs, st);
+      if constexpr (EPI == LS_ACT || EPI == LS_NORM || (EPI == LS_DACT && sizeof(T) == 2)) return ls_go<T, 16, EPI, DX, VEC>(a, n_slabs, st);
       break;                                                   // ls_bwd_max
   }
   set_error("linear_stream: %d channels", a.n);
