@@ -64,7 +64,7 @@ static LsArgs la_stream_args(const void* x, int64_t x_ld, const void* w, int64_t
   a.bias = bias; a.bias_dtype = bias_dtype; a.g = g; a.h = h; a.norm_dtype = norm_dtype;
   a.r = r; a.r_ld = r_ld;
   a.out = out;
-  a.vec = (k % (64 / es) == 0 && la_aligned(x, x_ld, es, 16) ? 1 : 0) | (n % 16 == 0 && la_aligned(r, r_ld, es, 4 * es) && la_aligned(out, n, es, 4 * es) ? 2 : 0);
+  a.vec = (k % (64 / es) == 0 && la_aligned(x, x_ld, es, 16) ? 1 : 0) | (n % 16 == 0 && la_aligned(r, r_ld, es, 16) && la_aligned(out, n, es, 16) ? 2 : 0);
   a.m = m; a.k = (int)k; a.n = (int)n; a.eps = (float)eps; a.act = act;
   return a;
 }
@@ -171,7 +171,7 @@ extern "C" int pygho_linear_act_bwd(void* gx, void* gw, int gw_dtype, void* gb, 
   char* base = reinterpret_cast<char*>(workspace);
   // (`out`: dz's place, aligned by its own rule; gx joins the condition because dX is stored in the same launch)
   LsArgs fa = la_stream_args(x, x_ld, w, w_ld, bias, bias_dtype, g, h, norm_dtype, gy, gy_ld, base, m_cap, k, n, eps, act, dtype);
-  if (gx && !(k % 16 == 0 && la_aligned(gx, k, es, 4 * es))) fa.vec &= 1;
+  if (gx && !(k % 16 == 0 && la_aligned(gx, k, es, 16))) fa.vec &= 1;
   fa.m_dev = m_dev;
   const LaSpace sp = la_space(m_cap, k, n, norm, act, dtype, fa.vec == 3);
   if (workspace_bytes < (size_t)sp.total || (uintptr_t)workspace % 16 != 0) { set_error("linear_act_bwd: workspace too small or not 16-byte aligned"); return PYGHO_ERR_INVALID; }

@@ -19,7 +19,7 @@ template <typename T, int KS> constexpr int lo_blocks() { return sizeof(T) == 4 
 template <typename T, int KS, int VEC>
 __global__ __launch_bounds__(kLoThreads) void linear_out_kernel(LsArgs a) {
   constexpr bool P = Precise<T>::value;
-  constexpr bool XV = VEC & 1, NV = VEC & 2;                   // as in linear_stream.h
+  constexpr bool XV = VEC & 1, NV = VEC & 2, PAIR = sizeof(T) == 2 && NV;      // as in linear_stream.h
   constexpr int ES = sizeof(T), E = 16 / ES, MB = lo_blocks<T, KS>(), PITCH = KS * 64 + 16;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int K = a.k, N = a.n, NP = (N + 15) & ~15;
@@ -87,13 +87,33 @@ __global__ __launch_bounds__(kLoThreads) void linear_out_kernel(LsArgs a) {
         for (int mb = 0; mb < MB; ++mb) {
           o[mb][t] = b4;
           rv[mb][t] = typename Raw4<T>::type{};
-          if (a.r) {
-            const uint32_t off = (uint32_t)min(mb * 16 + r16, last) * (uint32_t)(a.r_ld * ES);
-            if constexpr (NV) rv[mb][t] = *reinterpret_cast<const typename Raw4<T>::type*>(rbase + off + (nb + q * 4) * ES);
-            else rv[mb][t] = ls_load4<T>(reinterpret_cast<const T*>(rbase + off), nb + q * 4, N, 0);
-          }
         }
       }
+      auto load_r = [&]() {
+        if (!a.r) return;
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+          const uint32_t row = (uint32_t)min(mb * 16 + r16, last) * (uint32_t)(a.r_ld * ES);
+#pragma unroll
+          for (int t = 0; t < 4; t += 2) {
+            if constexpr (PAIR) {
+              if (n0 + t * 16 + 32 <= N) {
+                const uint4 v = *reinterpret_cast<const uint4*>(rbase + row + (n0 + t * 16 + ls_pair_col(q)) * ES);
+                rv[mb][t] = make_uint2(v.x, v.y);
+                rv[mb][t + 1] = make_uint2(v.z, v.w);
+                continue;
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int nb = min(n0 + (t + i) * 16, NP - 16);
+              if constexpr (NV) rv[mb][t + i] = *reinterpret_cast<const typename Raw4<T>::type*>(rbase + row + (nb + q * 4) * ES);
+              else rv[mb][t + i] = ls_load4<T>(reinterpret_cast<const T*>(rbase + row), nb + q * 4, N, 0);
+            }
+          }
+        }
+      };
+      if constexpr (KS < 8) load_r();                          // in flight during the products; with 8 steps of x there are no registers for it
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -103,20 +123,41 @@ __global__ __launch_bounds__(kLoThreads) void linear_out_kernel(LsArgs a) {
 #pragma unroll
           for (int mb = 0; mb < MB; ++mb) o[mb][t] = la_mfma<T>(fa, xc[mb][s], o[mb][t]);
         }
+      if constexpr (KS == 8) load_r();
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb) {
         const int rr = mb * 16 + r16;
+        const uint32_t row16 = (uint32_t)rr * (uint32_t)(N * ES), row32 = (uint32_t)rr * (uint32_t)(N * 4);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const int n = n0 + t * 16 + q * 4;
-          float u[4] = {o[mb][t][0], o[mb][t][1], o[mb][t][2], o[mb][t][3]}, r4[4];
-          ro_act<P, 4>(u, a.act);
-          ls_unpack4<T>(rv[mb][t], r4);
+        for (int t = 0; t < 4; t += 2) {
+          const bool pair = PAIR && n0 + t * 16 + 32 <= N;     // (uniform)
+          if constexpr (PAIR) { if (pair) ls_pair(rv[mb][t], rv[mb][t + 1]); }
+          float u[2][4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) u[e] += r4[e];
-          if (rr <= last && (NV ? n0 + t * 16 : n) < N) {
-            if (a.out_f32) la_store4<float>(reinterpret_cast<float*>(obase + (uint32_t)rr * (uint32_t)(N * 4) + n * 4), NV ? 4 : N - n, NV, u);
-            else la_store4<T>(reinterpret_cast<T*>(obase + (uint32_t)rr * (uint32_t)(N * ES) + n * ES), NV ? 4 : N - n, NV, u);
+          for (int i = 0; i < 2; ++i) {
+            float r4[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) u[i][e] = o[mb][t + i][e];
+            ro_act<P, 4>(u[i], a.act);
+            ls_unpack4<T>(rv[mb][t + i], r4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) u[i][e] += r4[e];
+          }
+          if constexpr (PAIR) {
+            if (pair && !a.out_f32) {
+              uint2 lo = ls_pack4<T>(u[0]), hi = ls_pack4<T>(u[1]);
+              ls_pair(lo, hi);
+              if (rr <= last) *reinterpret_cast<uint4*>(obase + row16 + (n0 + t * 16 + ls_pair_col(q)) * ES) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+              continue;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int n = n0 + (t + i) * 16 + q * 4;
+            if (rr <= last && (NV ? n0 + (t + i) * 16 : n) < N) {
+              if (a.out_f32) la_store4<float>(reinterpret_cast<float*>(obase + row32 + n * 4), NV ? 4 : N - n, NV, u[i]);
+              else la_store4<T>(reinterpret_cast<T*>(obase + row16 + n * ES), NV ? 4 : N - n, NV, u[i]);
+            }
           }
         }
       }

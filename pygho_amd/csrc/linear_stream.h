@@ -84,6 +84,22 @@ template <typename T> __device__ __forceinline__ void ls_unpack4(const typename 
   }
 }
 
+// 16-bit rows of whole 16-channel blocks: two neighbouring blocks' 4 channels per lane become 8 consecutive channels of one of them -- a swap of the odd
+// 16-lane groups of the first with the even ones of the second -- so that a load or store moves 64 contiguous bytes per row, not 2 x 32.  The swap
+// is its own inverse.  Lane (r16, q) then holds channels ls_pair_col(q) .. + 7 of the two blocks' 32
+__device__ __forceinline__ void ls_pair(uint2& a, uint2& b) {
+  auto r = __builtin_amdgcn_permlane16_swap(a.x, b.x, false, false);
+  a.x = r[0]; b.x = r[1];
+  r = __builtin_amdgcn_permlane16_swap(a.y, b.y, false, false);
+  a.y = r[0]; b.y = r[1];
+}
+__device__ __forceinline__ int ls_pair_col(int q) { return (q & 1) * 16 + (q >> 1) * 8; }
+template <typename T> __device__ __forceinline__ uint2 ls_pack4(const float (&v)[4]) {
+  const float t[8] = {v[0], v[1], v[2], v[3], 0.f, 0.f, 0.f, 0.f};
+  const uint4 r = Vec16<T>::pack(t);
+  return make_uint2(r.x, r.y);
+}
+
 // 8 16-bit values per lane out of a row-major LDS tile, transposed: lane r16 gets column r16 of 4 rows at p's 16 lanes and of 4 rows `dist` bytes on
 __device__ __forceinline__ uint4 ls_read_tr(const char* p, int dist) {
   const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) la_s4_t*)p));
@@ -114,8 +130,12 @@ template <int V, int S> __device__ __forceinline__ void ls_row_sums(float (&v)[V
 }
 
 // wavefronts per SIMD the registers are limited to (512 / this many per lane): latency, not throughput, is what a turn of 16 rows has most of
-// (the gradient through a norm of 65 .. 128 channels with the next block's rows in flight: 168 registers do not hold it)
-constexpr int ls_wps(int nb, int epi, int es) { return nb <= 4 ? (nb == 4 && es == 4 && epi == LS_DNORM ? 3 : 4) : nb <= 8 && epi != LS_DNORM ? 3 : 2; }
+// (fewer where they do not hold the kernel: the gradient through a norm of 65 .. 128 channels with the next block's rows in flight, and accesses
+// element by element with an address each)
+constexpr int ls_wps(int nb, int epi, int vec, int es) {
+  if (vec != 3) return nb <= 2 ? 4 : nb == 4 ? 3 : nb == 8 ? 2 : 1;
+  return nb <= 4 ? (nb == 4 && es == 4 && epi == LS_DNORM ? 3 : 4) : nb == 8 && epi != LS_DNORM ? 3 : 2;
+}
 
 // geometry that host and device share
 template <typename T, int NB> struct LsGeom {
@@ -135,14 +155,14 @@ template <typename T, int NB> struct LsGeom {
 constexpr int kLsDwWaves = 4;
 
 // VEC & 1: k is a whole number of 64-byte steps and x's rows allow 16-byte accesses.  VEC & 2: n is a whole number of 16 channels and the rows of r, out
-// and gx allow accesses of 4 elements (k of 16, with gx).  A block's rows then are one uniform base address, one 32-bit offset per lane and
+// and gx are on 16-byte boundaries (k of 16, with gx).  A block's rows then are one uniform base address, one 32-bit offset per lane and
 // constants -- 64-bit addresses per access, or masks per element, take more registers than the sums do.  Otherwise element by element.
 //
 // DW (16-bit, k <= 128): the weight gradient in the same launch.  The workgroup's wavefronts go through their blocks in step; each puts its dz
 // and its x (16 rows, row-major) into LDS, and after a barrier forms its share of dW += dz^T x over the 64 rows, both operands read back
 // transposed by the LDS (ds_read_b64_tr_b16).  dz never reaches memory and x is read once: 3 streams instead of 6
 template <typename T, int NB, int EPI, bool DX, int VEC, bool DW = false>
-__global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, sizeof(T)) * 256, DW ? 2 : ls_wps(NB, EPI, sizeof(T))) void linear_stream_kernel(LsArgs a) {
+__global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC, sizeof(T)) * 256, DW ? 2 : ls_wps(NB, EPI, VEC, sizeof(T))) void linear_stream_kernel(LsArgs a) {
   using G = LsGeom<T, NB>;
   constexpr bool P = Precise<T>::value, BWD = EPI == LS_DACT || EPI == LS_DNORM, NORM = EPI == LS_NORM || EPI == LS_DNORM;
   constexpr int ES = G::ES, E = 16 / ES, NP = G::NP, KC = 4;
@@ -256,22 +276,38 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, sizeof(T)
   typename Raw4<T>::type rv[NB];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) rv[nb] = typename Raw4<T>::type{};
-  constexpr bool AHEAD = !(ES == 4 && NB == 16);               // (256 f32 channels: 64 registers more than there are)
+  constexpr bool PAIR = ES == 2 && NV && NB > 1;
+  constexpr bool AHEAD = VEC == 3 && !(ES == 4 && NB == 16);   // (256 f32 channels, or addresses per element: more registers than there are)
   auto load_r = [&](int64_t b) {
     if (!a.r) return;
     b = min(b, n_blocks - 1);
     const char* base = reinterpret_cast<const char*>(a.r) + b * 16 * a.r_ld * ES;
-    const uint32_t off = (uint32_t)lane_row(b) * (uint32_t)(a.r_ld * ES) + (NV ? q * 4 * ES : 0);
+    const uint32_t row = (uint32_t)lane_row(b) * (uint32_t)(a.r_ld * ES), off = row + (NV ? q * 4 * ES : 0);
     int N_here = N;                                            // (compared here, not held as 16 masks for the whole loop)
     asm volatile("" : "+s"(N_here));
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      if constexpr (NV) {
-        if (nb * 16 < N_here) rv[nb] = *reinterpret_cast<const typename Raw4<T>::type*>(base + off + nb * 16 * ES);
-      } else {
-        rv[nb] = ls_load4<T>(reinterpret_cast<const T*>(base + off), nb * 16 + q * 4, N, 0);
+    for (int p = 0; p < NB; p += 2) {
+      if constexpr (PAIR) {
+        if ((p + 2) * 16 <= N_here) {
+          const uint4 v = *reinterpret_cast<const uint4*>(base + row + (p * 16 + ls_pair_col(q)) * ES);
+          rv[p] = make_uint2(v.x, v.y);
+          rv[p + 1] = make_uint2(v.z, v.w);
+          continue;
+        }
+      }
+#pragma unroll
+      for (int nb = p; nb < (p + 2 < NB ? p + 2 : NB); ++nb) {
+        if constexpr (NV) {
+          if (nb * 16 < N_here) rv[nb] = *reinterpret_cast<const typename Raw4<T>::type*>(base + off + nb * 16 * ES);
+        } else {
+          rv[nb] = ls_load4<T>(reinterpret_cast<const T*>(base + off), nb * 16 + q * 4, N, 0);
+        }
       }
     }
+  };
+  auto use_r = [&](int nb, float (&v)[4]) {                    // (called for nb = 0, 1, ..)
+    if constexpr (PAIR) { if (nb % 2 == 0 && (nb + 2) * 16 <= N) ls_pair(rv[nb], rv[nb + 1 < NB ? nb + 1 : 0]); }
+    ls_unpack4<T>(rv[nb], v);
   };
   if ((DW ? blk - wave : blk) < n_blocks) {
     load_x(blk, 0, xc);
@@ -302,8 +338,10 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, sizeof(T)
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) acc[nb] = *reinterpret_cast<const la_f32x4_t*>(lds_bias + nb * 16 + q * 4);
     for (int kc = 0; kc < nk; ++kc) {
-      if (kc + 1 < nk) load_x(blk, kc + 1, xn);
-      else load_x(min(blk + stride, n_blocks - 1), 0, xn);
+      if constexpr (!DW) {
+        if (kc + 1 < nk) load_x(blk, kc + 1, xn);
+        else load_x(min(blk + stride, n_blocks - 1), 0, xn);
+      }
 #pragma unroll
       for (int s = 0; s < KC; ++s) {
         if (kc * KC + s < KS) {
@@ -314,8 +352,12 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, sizeof(T)
           }
         }
       }
+      if constexpr (DW) {                                      // (k <= 128: one step of the loop, the registers are free for the next block)
+        load_x(blk + stride, 0, xc);
+      } else {
 #pragma unroll
-      for (int s = 0; s < KC; ++s) xc[s] = xn[s];
+        for (int s = 0; s < KC; ++s) xc[s] = xn[s];
+      }
     }
     {
       float v[NB][4], rstd = 0.f;
@@ -354,11 +396,23 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, sizeof(T)
       auto store_rows = [&](auto* rows, float (&val)[NB][4], int64_t width) {
         using O = std::remove_reference_t<decltype(*rows)>;
         char* base = reinterpret_cast<char*>(rows) + blk * 16 * width * (int64_t)sizeof(O);
-        const uint32_t off = (uint32_t)r16 * (uint32_t)(width * sizeof(O)) + q * 4 * sizeof(O);
+        const uint32_t row = (uint32_t)r16 * (uint32_t)(width * sizeof(O));
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-          if ((NV ? nb * 16 : nb * 16 + q * 4) < N_here)
-            la_store4<O>(reinterpret_cast<O*>(base + off + nb * 16 * sizeof(O)), NV ? 4 : N - nb * 16 - q * 4, NV, val[nb]);
+        for (int nb = 0; nb < NB; nb += 2) {
+          if constexpr (PAIR && sizeof(O) == 2) {
+            if ((nb + 2) * 16 <= N_here) {
+              uint2 lo = ls_pack4<T>(val[nb]), hi = ls_pack4<T>(val[nb + 1 < NB ? nb + 1 : nb]);
+              ls_pair(lo, hi);                                 // (before the rows past the end drop out: every lane takes part)
+              if (row_ok) *reinterpret_cast<uint4*>(base + row + (nb * 16 + ls_pair_col(q)) * 2) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+              continue;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 2 && nb + i < NB; ++i) {
+            const int n = (nb + i) * 16 + q * 4;
+            if (row_ok && (NV ? (nb + i) * 16 : n) < N_here) la_store4<O>(reinterpret_cast<O*>(base + row + n * sizeof(O)), NV ? 4 : N - n, NV, val[nb + i]);
+          }
+        }
       };
       // (channel block by channel block: whole-row arrays of intermediates do not fit beside the sums and the next block's x)
       if constexpr (!BWD) {
@@ -372,21 +426,19 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, sizeof(T)
           }
           ro_act<P, 4>(v[nb], a.act);
           float r4[4];
-          ls_unpack4<T>(rv[nb], r4);
+          use_r(nb, r4);
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[nb][e] += r4[e];
         }
         if constexpr (AHEAD) load_r(blk + stride);
-        if (row_ok) {
-          if (EPI == LS_ACT && a.out_f32) store_rows(reinterpret_cast<float*>(a.out), v, N);
-          else store_rows(reinterpret_cast<T*>(a.out), v, N);
-        }
+        if (EPI == LS_ACT && a.out_f32) store_rows(reinterpret_cast<float*>(a.out), v, N);
+        else store_rows(reinterpret_cast<T*>(a.out), v, N);
       } else {
         float d[NB][4], k1 = 0.f, k2 = 0.f;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
           const int n = nb * 16 + q * 4;
-          ls_unpack4<T>(rv[nb], d[nb]);
+          use_r(nb, d[nb]);
           if constexpr (NORM) {
             const float4 g4 = *reinterpret_cast<const float4*>(lds_g + n);
             const float gv[4] = {g4.x, g4.y, g4.z, g4.w};
@@ -437,7 +489,7 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, sizeof(T)
           for (int i = 0; i < NB * 4; ++i) t[i] = d[i / 4][i % 4];
           add_rows(NSUM ? NSUM - 1 : 0, t);
         }
-        if (!DW && row_ok) store_rows(reinterpret_cast<T*>(a.out), d, N);
+        if constexpr (!DW) store_rows(reinterpret_cast<T*>(a.out), d, N);
         if constexpr (!DX && AHEAD) load_r(blk + stride);
         if constexpr (DX) {
           // dz as the operand of dz . W: step s of n = this lane's registers 2 s, 2 s + 1 (16-bit, rounded once) or s (f32)
@@ -453,7 +505,7 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, sizeof(T)
               f[s] = Vec16<T>::pack(t);
             }
           }
-          if constexpr (AHEAD) load_r(blk + stride);                                // (xh and dz have left their registers)
+          if constexpr (AHEAD && !DW) load_r(blk + stride);    // (xh and dz have left their registers)
           if constexpr (DW) {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
@@ -476,8 +528,9 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, sizeof(T)
               }
             }
           }
+          if constexpr (DW) load_r(blk + stride);
           char* base = reinterpret_cast<char*>(a.gx) + blk * 16 * K * ES;
-          const uint32_t off = (uint32_t)r16 * (uint32_t)(K * ES) + q * 4 * ES;
+          const uint32_t row = (uint32_t)r16 * (uint32_t)(K * ES);
           const int kb_end = DW && !a.gx ? 0 : (K + 15) / 16;
           constexpr int KG = NORM ? 2 : 4;                     // 16-channel blocks at once (the norm's registers leave room for two)
           for (int kg = 0; kg < kb_end; kg += KG) {
@@ -495,10 +548,22 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, sizeof(T)
                 o[t] = la_mfma<T>(fa, f[s], o[t]);
               }
 #pragma unroll
-            for (int t = 0; t < KG; ++t) {
-              const int k = (kg + t) * 16 + q * 4;
-              const float o4[4] = {o[t][0], o[t][1], o[t][2], o[t][3]};
-              if (row_ok && k < K) la_store4<T>(reinterpret_cast<T*>(base + (kg + t) * 16 * ES + off), NV ? 4 : K - k, NV, o4);
+            for (int t = 0; t < KG; t += 2) {
+              if constexpr (ES == 2 && NV) {
+                if ((kg + t + 2) * 16 <= K) {
+                  const float l4[4] = {o[t][0], o[t][1], o[t][2], o[t][3]}, h4[4] = {o[t + 1][0], o[t + 1][1], o[t + 1][2], o[t + 1][3]};
+                  uint2 lo = ls_pack4<T>(l4), hi = ls_pack4<T>(h4);
+                  ls_pair(lo, hi);
+                  if (row_ok) *reinterpret_cast<uint4*>(base + row + ((kg + t) * 16 + ls_pair_col(q)) * 2) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+                  continue;
+                }
+              }
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const int k = (kg + t + i) * 16 + q * 4;
+                const float o4[4] = {o[t + i][0], o[t + i][1], o[t + i][2], o[t + i][3]};
+                if (row_ok && k < K) la_store4<T>(reinterpret_cast<T*>(base + row + k * ES), NV ? 4 : K - k, NV, o4);
+              }
             }
           }
         }
@@ -548,7 +613,7 @@ constexpr int ls_nb(int64_t n) { return n <= 16 ? 1 : n <= 32 ? 2 : n <= 64 ? 4 
 
 template <typename T, int NB> static int ls_red(int k, int sums) {      // W, and at the end the wavefronts' sums in its place
   using G = LsGeom<T, NB>;
-  return std::max(G::w_bytes(k), ls_wps(NB, LS_ACT, sizeof(T)) * 4 * sums * G::NP * 4);
+  return std::max(G::w_bytes(k), ls_wps(NB, LS_ACT, 3, sizeof(T)) * 4 * sums * G::NP * 4);
 }
 template <typename T, int NB> static int ls_lds(int k, int sums, bool dx, bool dw = false) {
   using G = LsGeom<T, NB>;
@@ -576,7 +641,7 @@ constexpr int ls_bwd_max(int norm, int elem_size) { return norm || elem_size == 
 constexpr int kLsGrid = 1024;                                  // most workgroups of a launch (and slabs)
 
 template <typename T, int NB, int EPI, bool DX, int VEC, bool DW = false> static int ls_go(LsArgs a, int* n_slabs, hipStream_t st) {
-  constexpr int NSUM = EPI == LS_DNORM ? 3 : EPI == LS_DACT ? 1 : 0, WPS = ls_wps(NB, EPI, sizeof(T));
+  constexpr int NSUM = EPI == LS_DNORM ? 3 : EPI == LS_DACT ? 1 : 0, WPS = ls_wps(NB, EPI, VEC, sizeof(T));
   const int lds = ls_lds<T, NB>(a.k, NSUM, DX, DW);
   a.red_bytes = ls_red<T, NB>(a.k, NSUM);
   static bool attr_set_dev[64] = {};
