@@ -11,7 +11,7 @@ namespace pygho {
   template <> int LinearOps<T>::out_fwd(const LsArgs&, hipStream_t);                          \
   template <> int LinearOps<T>::stream_bwd(const LsArgs&, int, bool, int*, hipStream_t);      \
   template <> int LinearOps<T>::tile_act(const LaArgs&, hipStream_t);                         \
-  template <> int LinearOps<T>::tile_dx(const LaArgs&, hipStream_t);                          \
+  template <> int LinearOps<T>::transpose(void*, const void*, int64_t, int64_t, int64_t, hipStream_t); \
   template <> int LinearOps<T>::tile_dw(const LaArgs&, hipStream_t);
 PYGHO_LINEAR_DECL(float)
 PYGHO_LINEAR_DECL(bf16)
@@ -91,11 +91,11 @@ static int64_t la_dw_slabs(int64_t m, int64_t k, int64_t n) {
 }
 static int64_t la_pad4(int64_t v) { return (v + 3) / 4 * 4; }
 
-// The launches of a backward pass and its workspace, in bytes: [dz] [z] [slabs of the sums over n] [slabs of dW | db]
+// The launches of a backward pass and its workspace, in bytes: [dz] [z] [slabs of the sums over n] [slabs of dW | db] [W^T]
 //   fused   dz, dX, dW and every sum from one streaming launch (operands aligned; its slabs are [sums | dW])
 //   stream  dz with the sums (and dX where both copies of W fit) from a streaming launch
 //   else    dz by the row kernel from the pre-activation: kept by the forward, or (z) formed again in f32 where the forward streams
-struct LaSpace { int64_t dz, z, sums, dw, total; int nsum; bool fused, stream, own_dz; };
+struct LaSpace { int64_t dz, z, sums, dw, wt, total; int nsum; bool fused, stream, own_dz; };
 static LaSpace la_space(int64_t m, int64_t k, int64_t n, int norm, int act, int dtype, bool aligned) {
   LaSpace s{};
   s.nsum = norm ? 3 : 1;
@@ -110,7 +110,8 @@ static LaSpace la_space(int64_t m, int64_t k, int64_t n, int norm, int act, int 
   s.z = s.own_dz && !s.stream && la_form(k, n, norm, dtype) != FORM_TILE ? (m * n * 4 + 15) / 16 * 16 : 0;
   s.sums = !s.own_dz ? 0 : s.stream ? kLsGrid * la_pad4(s.nsum * n) * 4 : ln_bwd_slab_floats(m, n, s.nsum) * 4;
   s.dw = la_dw_slabs(m, k, n) * la_pad4(n * k + n) * 4;
-  s.total = s.dz + s.z + s.sums + s.dw;
+  s.wt = la_form(n, k, 0, dtype) == FORM_TILE ? (n * k * la_size(dtype) + 15) / 16 * 16 : 0;
+  s.total = s.dz + s.z + s.sums + s.dw + s.wt;
   return s;
 }
 
@@ -227,12 +228,9 @@ extern "C" int pygho_linear_act_bwd(void* gx, void* gw, int gw_dtype, void* gb, 
       a.w_trans = 1;
       if (int rc = la_forward(a, form, 0, dtype, st)) return rc;
     } else {
-      LaArgs a{};
-      a.a = la_operand(dz, dz_ld, dtype);
-      a.b = la_operand(w, w_ld, dtype);
-      a.m = m_cap; a.n = k; a.k = n;
-      a.out = gx; a.out_vec = la_aligned(gx, k, es, 4 * es);
-      if (int rc = la_type(dtype, [&](auto ops) { return ops.tile_dx(a, st); })) return rc;
+      void* wt = base + sp.dz + sp.z + sp.sums + sp.dw;
+      if (int rc = la_type(dtype, [&](auto ops) { return ops.transpose(wt, w, w_ld, n, k, st); })) return rc;
+      if (int rc = la_tile_act(dz, dz_ld, wt, n, nullptr, 0, nullptr, 0, gx, nullptr, 0, m_cap, n, k, kActNone, dtype, st)) return rc;
     }
   }
   const bool db_here = gb && !sp.own_dz;                      // dz is gy itself: its column sums come with dW

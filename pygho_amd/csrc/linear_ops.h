@@ -14,7 +14,7 @@ template <typename T> struct LinearOps {
   static int out_fwd(const LsArgs& a, hipStream_t st);
   static int stream_bwd(const LsArgs& a, int norm, bool dw, int* n_slabs, hipStream_t st);
   static int tile_act(const LaArgs& a, hipStream_t st);
-  static int tile_dx(const LaArgs& a, hipStream_t st);
+  static int transpose(void* wt, const void* w, int64_t w_ld, int64_t n, int64_t k, hipStream_t st);
   static int tile_dw(const LaArgs& a, hipStream_t st);
 };
 
@@ -32,7 +32,9 @@ template <typename T> struct LinearOps {
     return norm ? ls_pick<T, LS_DNORM, false>(a, n_slabs, st) : ls_pick<T, LS_DACT, false>(a, n_slabs, st);                                    \
   }                                                                                                                                            \
   template <> int LinearOps<T>::tile_act(const LaArgs& a, hipStream_t st) { return la_any<T, LA_ROWS, LA_ROWS, LA_ACT>(a, st); }               \
-  template <> int LinearOps<T>::tile_dx(const LaArgs& a, hipStream_t st) { return la_any<T, LA_ROWS, LA_COLS, LA_ACT>(a, st); }                \
+  template <> int LinearOps<T>::transpose(void* wt, const void* w, int64_t w_ld, int64_t n, int64_t k, hipStream_t st) {                       \
+    return la_transpose<T>(wt, w, w_ld, n, k, st);                                                                                             \
+  }                                                                                                                                            \
   template <> int LinearOps<T>::tile_dw(const LaArgs& a, hipStream_t st) { return la_any<T, LA_COLS, LA_COLS, LA_SLAB>(a, st); }
 
 }  // namespace pygho

@@ -277,6 +277,7 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC, size
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) rv[nb] = typename Raw4<T>::type{};
   constexpr bool PAIR = ES == 2 && NV && NB > 1;
+  constexpr bool PAIR_R = PAIR && !DW;                         // (in the fused gradient the swap comes in front of everything: 0.60 against 0.53 ms)
   constexpr bool AHEAD = VEC == 3 && !(ES == 4 && NB == 16);   // (256 f32 channels, or addresses per element: more registers than there are)
   auto load_r = [&](int64_t b) {
     if (!a.r) return;
@@ -287,7 +288,7 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC, size
     asm volatile("" : "+s"(N_here));
 #pragma unroll
     for (int p = 0; p < NB; p += 2) {
-      if constexpr (PAIR) {
+      if constexpr (PAIR_R) {
         if ((p + 2) * 16 <= N_here) {
           const uint4 v = *reinterpret_cast<const uint4*>(base + row + (p * 16 + ls_pair_col(q)) * ES);
           rv[p] = make_uint2(v.x, v.y);
@@ -306,7 +307,7 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC, size
     }
   };
   auto use_r = [&](int nb, float (&v)[4]) {                    // (called for nb = 0, 1, ..)
-    if constexpr (PAIR) { if (nb % 2 == 0 && (nb + 2) * 16 <= N) ls_pair(rv[nb], rv[nb + 1 < NB ? nb + 1 : 0]); }
+    if constexpr (PAIR_R) { if (nb % 2 == 0 && (nb + 2) * 16 <= N) ls_pair(rv[nb], rv[nb + 1 < NB ? nb + 1 : 0]); }
     ls_unpack4<T>(rv[nb], v);
   };
   if ((DW ? blk - wave : blk) < n_blocks) {
@@ -435,26 +436,39 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC, size
         else store_rows(reinterpret_cast<T*>(a.out), v, N);
       } else {
         float d[NB][4], k1 = 0.f, k2 = 0.f;
+        constexpr int GB = NB >= 8 ? 2 : 1;                    // channel blocks per activation switch
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          const int n = nb * 16 + q * 4;
-          use_r(nb, d[nb]);
+        for (int n0 = 0; n0 < NB; n0 += GB) {
+#pragma unroll
+          for (int i = 0; i < GB; ++i) use_r(n0 + i, d[n0 + i]);
+          if (a.act != kActNone) {
+            float z[GB][4];
+#pragma unroll
+            for (int i = 0; i < GB; ++i) {
+              if constexpr (NORM) {
+                const int n = (n0 + i) * 16 + q * 4;
+                const float4 g4 = *reinterpret_cast<const float4*>(lds_g + n), h4 = *reinterpret_cast<const float4*>(lds_h + n);
+                z[i][0] = fmaf(v[n0 + i][0], g4.x, h4.x); z[i][1] = fmaf(v[n0 + i][1], g4.y, h4.y);
+                z[i][2] = fmaf(v[n0 + i][2], g4.z, h4.z); z[i][3] = fmaf(v[n0 + i][3], g4.w, h4.w);
+              } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) z[i][e] = v[n0 + i][e];
+              }
+            }
+            ro_act_slope<P, GB * 4>(reinterpret_cast<float(&)[GB * 4]>(d[n0]), reinterpret_cast<const float(&)[GB * 4]>(z), a.act);
+          }
           if constexpr (NORM) {
-            const float4 g4 = *reinterpret_cast<const float4*>(lds_g + n);
-            const float gv[4] = {g4.x, g4.y, g4.z, g4.w};
-            if (a.act != kActNone) {
-              const float4 h4 = *reinterpret_cast<const float4*>(lds_h + n);
-              const float z[4] = {fmaf(v[nb][0], g4.x, h4.x), fmaf(v[nb][1], g4.y, h4.y), fmaf(v[nb][2], g4.z, h4.z), fmaf(v[nb][3], g4.w, h4.w)};
-              ro_act_slope<P, 4>(d[nb], z, a.act);
-            }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float ev = d[nb][e] * gv[e];
-              k1 += ev;
-              k2 = fmaf(ev, v[nb][e], k2);
+            for (int i = 0; i < GB; ++i) {
+              const float4 g4 = *reinterpret_cast<const float4*>(lds_g + (n0 + i) * 16 + q * 4);
+              const float gv[4] = {g4.x, g4.y, g4.z, g4.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float ev = d[n0 + i][e] * gv[e];
+                k1 += ev;
+                k2 = fmaf(ev, v[n0 + i][e], k2);
+              }
             }
-          } else {
-            if (a.act != kActNone) ro_act_slope<P, 4>(d[nb], v[nb], a.act);
           }
         }
         if constexpr (NORM) {
@@ -505,7 +519,7 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC, size
               f[s] = Vec16<T>::pack(t);
             }
           }
-          if constexpr (AHEAD && !DW) load_r(blk + stride);    // (xh and dz have left their registers)
+          if constexpr (AHEAD) load_r(blk + stride);           // (xh and dz have left their registers)
           if constexpr (DW) {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
@@ -528,7 +542,6 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC, size
               }
             }
           }
-          if constexpr (DW) load_r(blk + stride);
           char* base = reinterpret_cast<char*>(a.gx) + blk * 16 * K * ES;
           const uint32_t row = (uint32_t)r16 * (uint32_t)(K * ES);
           const int kb_end = DW && !a.gx ? 0 : (K + 15) / 16;

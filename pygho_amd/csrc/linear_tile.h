@@ -1,7 +1,7 @@
 // Tiled product behind the linear operators where W does not fit a CU's LDS (linear_stream.h is the other form), and for the weight
 // gradient, whose long dimension is the reduction.  Any width, row stride, alignment, f32 / bf16 / f16.
 // Output element (m, n) = sum_k P(m, k) Q(n, k); an operand is stored with its k contiguous ("rows": x and W of the forward, dz of dX) or
-// with its m / n contiguous ("columns": W of dX, dz and x of dW).  A step of the k loop moves 128 bytes of k per row (64 16-bit or 32 f32
+// with its m / n contiguous ("columns": dz and x of dW; dX takes W's transposed copy, which costs less than reading it transposed tile by tile).  A step of the k loop moves 128 bytes of k per row (64 16-bit or 32 f32
 // values) global -> registers -> LDS, one step ahead of the matrix instructions.  The MFMA runs in the swapped form D[n][m]: a lane holds one
 // row m and 4 consecutive n, which it stores as one vector.
 // Column operands stay in their storage order in LDS; 16-bit fragments are read back transposed by the LDS itself (ds_read_b64_tr_b16),
@@ -62,7 +62,7 @@ __device__ __forceinline__ float la_q_sum(float v) {     // over the 4 lanes of 
 }
 
 // geometry of an operand tile of R rows x 128 bytes of k in LDS
-template <typename T, int MODE, int R> struct LaTile {
+template <typename T, int MODE, int R, int THREADS> struct LaTile {
   static constexpr int ES = sizeof(T);
   static constexpr int KE = 128 / ES;                                            // k values per step of the loop
   // + 16 bytes per row: the 16 rows of a fragment read fall on different banks.  Columns: + 32 (16-bit: the 4 k rows of a transposed read)
@@ -70,15 +70,15 @@ template <typename T, int MODE, int R> struct LaTile {
   static constexpr int PITCH = MODE == LA_ROWS ? 128 + 16 : R * ES + (ES == 2 ? 32 : 16);
   static constexpr int BYTES = MODE == LA_ROWS ? R * PITCH : KE * PITCH;
   static constexpr int CHUNKS = R * 8;                                           // 16-byte chunks per step
-  static constexpr int PER_THREAD = (CHUNKS + kBlock - 1) / kBlock;
+  static constexpr int PER_THREAD = (CHUNKS + THREADS - 1) / THREADS;
   static constexpr int CPR = MODE == LA_ROWS ? 8 : R * ES / 16;                  // chunks per LDS row
 
   // chunk `i` of this thread: rows [r0, r0 + R) x k [k0, k0 + KE) of the operand; everything outside (n_rows, k_end) is zero
   static __device__ __forceinline__ uint4 load(const LaOperand& op, int64_t r0, int64_t n_rows, int64_t k0, int64_t k_end, int i) {
     constexpr int E = 16 / ES;
-    const int c = i * kBlock + (int)threadIdx.x;
+    const int c = i * THREADS + (int)threadIdx.x;
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (CHUNKS % kBlock != 0 && c >= CHUNKS) return v;
+    if (CHUNKS % THREADS != 0 && c >= CHUNKS) return v;
     const int lr = c / CPR, lc = c % CPR;
     const T* base = reinterpret_cast<const T*>(op.p);
     // `outer` runs over LDS rows, `inner` is the contiguous direction
@@ -101,9 +101,17 @@ template <typename T, int MODE, int R> struct LaTile {
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
+  // aligned rows and whole steps of k (FULL): one uniform base and 32-bit offsets; a row past the end repeats the last one (its products are not stored)
+  static __device__ __forceinline__ uint4 load_full(const LaOperand& op, int64_t r0, int64_t n_rows, int64_t k0, int i) {
+    static_assert(MODE == LA_ROWS && CHUNKS % THREADS == 0, "row operands");
+    const char* base = reinterpret_cast<const char*>(op.p) + (r0 * op.ld + k0) * ES;
+    const int last = (int)min((int64_t)(R - 1), n_rows - 1 - r0);
+    return *reinterpret_cast<const uint4*>(base + (uint32_t)min(i * (THREADS / 8) + (int)threadIdx.x / 8, last) * (uint32_t)(op.ld * ES) +
+                                           ((int)threadIdx.x % 8) * 16);
+  }
   static __device__ __forceinline__ void store(char* lds, const uint4& v, int i) {
-    const int c = i * kBlock + (int)threadIdx.x;
-    if (CHUNKS % kBlock != 0 && c >= CHUNKS) return;
+    const int c = i * THREADS + (int)threadIdx.x;
+    if (CHUNKS % THREADS != 0 && c >= CHUNKS) return;
     *reinterpret_cast<uint4*>(lds + (c / CPR) * PITCH + (c % CPR) * 16) = v;
   }
   // the lane's 16 bytes of k of row `row0 + lane % 16` in half-step ks (0, 1)
@@ -158,14 +166,14 @@ template <typename T> __device__ __forceinline__ void la_store4(T* p, int left, 
   }
 }
 
-// a workgroup of 4 wavefronts (WM x WN) forms BM x BN output tiles
-template <typename T, int MA, int MB, int BM, int BN, int WM, int WN, int EPI>
-__global__ __launch_bounds__(kBlock) void linear_tile_kernel(LaArgs g) {
-  using TA = LaTile<T, MA, BM>;
-  using TB = LaTile<T, MB, BN>;
+// a workgroup of WM x WN wavefronts forms BM x BN output tiles
+template <typename T, int MA, int MB, int BM, int BN, int WM, int WN, int EPI, bool FULL = false>
+__global__ __launch_bounds__(WM * WN * 64) void linear_tile_kernel(LaArgs g) {
+  using TA = LaTile<T, MA, BM, WM * WN * 64>;
+  using TB = LaTile<T, MB, BN, WM * WN * 64>;
   constexpr int KE = TA::KE, TM = BM / WM, TN = BN / WN, NM = TM / 16, NN = TN / 16;
   constexpr bool P = Precise<T>::value;
-  static_assert(WM * WN * kWave == kBlock && TM % 16 == 0 && TN % 16 == 0, "tile");
+  static_assert(TM % 16 == 0 && TN % 16 == 0, "tile");
   __shared__ __attribute__((aligned(16))) char lds_a[TA::BYTES];
   __shared__ __attribute__((aligned(16))) char lds_b[TB::BYTES];
   const int lane = threadIdx.x & 63, wave = PYGHO_WAVE_INDEX(threadIdx.x >> 6);
@@ -201,11 +209,18 @@ __global__ __launch_bounds__(kBlock) void linear_tile_kernel(LaArgs g) {
       return it * KE;
     };
     uint4 ra[TA::PER_THREAD], rb[TB::PER_THREAD];
-    auto fetch = [&](int64_t k0) {
+    auto fetch = [&](int64_t k0) __attribute__((always_inline)) {
+      if constexpr (FULL) {
 #pragma unroll
-      for (int i = 0; i < TA::PER_THREAD; ++i) ra[i] = TA::load(g.a, m0, m_rows, k0, k_end, i);
+        for (int i = 0; i < TA::PER_THREAD; ++i) ra[i] = TA::load_full(g.a, m0, m_rows, k0, i);
 #pragma unroll
-      for (int i = 0; i < TB::PER_THREAD; ++i) rb[i] = TB::load(g.b, n0, g.n, k0, k_end, i);
+        for (int i = 0; i < TB::PER_THREAD; ++i) rb[i] = TB::load_full(g.b, n0, g.n, k0, i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < TA::PER_THREAD; ++i) ra[i] = TA::load(g.a, m0, m_rows, k0, k_end, i);
+#pragma unroll
+        for (int i = 0; i < TB::PER_THREAD; ++i) rb[i] = TB::load(g.b, n0, g.n, k0, k_end, i);
+      }
     };
     la_f32x4_t acc[NM][NN], ones_acc[EPI == LA_SLAB ? NM : 1];
 #pragma unroll
@@ -217,7 +232,7 @@ __global__ __launch_bounds__(kBlock) void linear_tile_kernel(LaArgs g) {
       for (int i = 0; i < NM; ++i) ones_acc[i] = la_f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
     const bool sums = EPI == LA_SLAB && g.want_sums && n0 == 0 && wn == 0;
-    if (n_it > 0) fetch(k_of(0));
+    if (FULL || n_it > 0) fetch(k_of(0));                      // (FULL: k is at least one step)
     for (int64_t it = 0; it < n_it; ++it) {
       __syncthreads();                                   // the previous step's fragments are read
 #pragma unroll
@@ -225,18 +240,19 @@ __global__ __launch_bounds__(kBlock) void linear_tile_kernel(LaArgs g) {
 #pragma unroll
       for (int i = 0; i < TB::PER_THREAD; ++i) TB::store(lds_b, rb[i], i);
       __syncthreads();
-      if (it + 1 < n_it) fetch(k_of(it + 1));
+      if constexpr (FULL) fetch(k_of(min(it + 1, n_it - 1)));   // (unconditional: the registers stay registers)
+      else if (it + 1 < n_it) fetch(k_of(it + 1));
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
-        uint4 fm[NM], fn[NN];
+        uint4 fm[NM];
 #pragma unroll
         for (int i = 0; i < NM; ++i) fm[i] = TA::frag(lds_a, wm + i * 16, ks, r16, q);
 #pragma unroll
-        for (int j = 0; j < NN; ++j) fn[j] = TB::frag(lds_b, wn + j * 16, ks, r16, q);
+        for (int j = 0; j < NN; ++j) {
+          const uint4 fn = TB::frag(lds_b, wn + j * 16, ks, r16, q);
 #pragma unroll
-        for (int j = 0; j < NN; ++j)
-#pragma unroll
-          for (int i = 0; i < NM; ++i) acc[i][j] = la_mfma<T>(fn[j], fm[i], acc[i][j]);
+          for (int i = 0; i < NM; ++i) acc[i][j] = la_mfma<T>(fn, fm[i], acc[i][j]);
+        }
         if (sums) {                                      // column sums of dz: the same fragments against ones
 #pragma unroll
           for (int i = 0; i < NM; ++i) ones_acc[i] = la_mfma<T>(la_ones<T>(), fm[i], ones_acc[i]);
@@ -296,12 +312,27 @@ __global__ __launch_bounds__(kBlock) void linear_tile_kernel(LaArgs g) {
   }
 }
 
+// wt (k, n) = w (n, k) transposed: 32 x 32 tiles through LDS
+template <typename T> __global__ __launch_bounds__(kBlock) void la_transpose_kernel(T* __restrict__ wt, const T* __restrict__ w, int64_t w_ld, int64_t n, int64_t k) {
+  __shared__ T tile[32][33];
+  const int64_t n0 = (int64_t)blockIdx.y * 32, k0 = (int64_t)blockIdx.x * 32;
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  for (int i = ty; i < 32; i += 8) if (n0 + i < n && k0 + tx < k) tile[i][tx] = w[(n0 + i) * w_ld + k0 + tx];
+  __syncthreads();
+  for (int i = ty; i < 32; i += 8) if (k0 + i < k && n0 + tx < n) wt[(k0 + i) * n + n0 + tx] = tile[tx][i];
+}
+template <typename T> static int la_transpose(void* wt, const void* w, int64_t w_ld, int64_t n, int64_t k, hipStream_t st) {
+  if (ceil_div(n, 32) > 65535) { set_error("linear: %lld output channels", (long long)n); return PYGHO_ERR_UNSUPPORTED; }
+  hipLaunchKernelGGL((la_transpose_kernel<T>), dim3((unsigned)ceil_div(k, 32), (unsigned)ceil_div(n, 32)), dim3(kBlock), 0, st, (T*)wt, (const T*)w, w_ld, n, k);
+  return check_launch("linear_transpose");
+}
+
 static bool la_aligned(const void* p, int64_t ld, int es, int bytes) { return ((uintptr_t)p % bytes) == 0 && (ld * es) % bytes == 0; }
 
-template <typename T, int MA, int MB, int BM, int BN, int WM, int WN, int EPI> static int la_go(const LaArgs& a, int grid_cap, hipStream_t st) {
+template <typename T, int MA, int MB, int BM, int BN, int WM, int WN, int EPI, bool FULL = false> static int la_go(const LaArgs& a, int grid_cap, hipStream_t st) {
   const int64_t tiles = ceil_div(a.m, BM) * ceil_div(a.n, BN) * (EPI == LA_SLAB ? a.splits : 1);
   const int grid = (int)std::min<int64_t>((tiles + 7) / 8 * 8, grid_cap);
-  hipLaunchKernelGGL((linear_tile_kernel<T, MA, MB, BM, BN, WM, WN, EPI>), dim3(grid), dim3(kBlock), 0, st, a);
+  hipLaunchKernelGGL((linear_tile_kernel<T, MA, MB, BM, BN, WM, WN, EPI, FULL>), dim3(grid), dim3(WM * WN * 64), 0, st, a);
   return check_launch("linear_tile");
 }
 
@@ -312,6 +343,9 @@ template <typename T, int MA, int MB, int EPI> static int la_any(const LaArgs& a
   const int64_t sp = EPI == LA_SLAB ? a.splits : 1;
   auto count = [&](int bm, int bn) { return ceil_div(a.m, bm) * ceil_div(a.n, bn) * sp; };
   if (a.n <= 16) return la_go<T, MA, MB, 64, 16, 4, 1, EPI>(a, kLaGrid, st);
+  // 16-bit products large enough for a 256 x 256 tile per CU: a wavefront's 128 x 64 part reads 12 fragments of LDS per 32 MFMAs, a 64 x 64 part 8 per 16
+  if constexpr (sizeof(T) == 2 && EPI == LA_ACT)
+    if (a.n > 128 && count(256, 256) >= 256 && a.a.vec && a.b.vec && a.k % 64 == 0) return la_go<T, MA, MB, 256, 256, 2, 4, EPI, true>(a, kLaGrid, st);
   if (a.n > 64 && a.m > 64 && count(128, 128) >= 256) return la_go<T, MA, MB, 128, 128, 2, 2, EPI>(a, kLaGrid, st);
   return la_go<T, MA, MB, 64, 64, 2, 2, EPI>(a, kLaGrid, st);
 }
