@@ -203,11 +203,16 @@ act_dict = {"relu": nn.ReLU(inplace=True), "ELU": nn.ELU(inplace=True), "silu": 
 
 class MLP(nn.Module):
     """``numlayer`` x [Linear -> norm -> dropout -> act]; the last block only has norm/act when
-    ``tailact`` (reference utils.py:85-142; layer order inside ``lins`` is identical)."""
+    ``tailact`` (reference utils.py:85-142; layer order inside ``lins`` is identical).
+
+    ``fused`` (an extension, same parameters and ``state_dict``): on device tensors every [Linear, LayerNorm | none, act] run is one operator
+    (``_ops.linear_norm_act`` / ``_ops.linear_act``), the residual of ``forward`` included.  Under autocast such a block computes in the
+    autocast dtype from end to end (the stock modules return f32 from a LayerNorm); BatchNorm blocks are the same with and without it."""
 
     def __init__(self, hiddim: int, outdim: int, numlayer: int, tailact: bool, dp: float = 0, norm: str = "bn",
-                 act: str = "relu", tailbias=True, normparam: float = 0.1) -> None:
+                 act: str = "relu", tailbias=True, normparam: float = 0.1, fused: bool = False) -> None:
         super().__init__()
+        self.fused = bool(fused)
         assert numlayer >= 0
         if numlayer == 0:
             assert hiddim == outdim
@@ -258,6 +263,8 @@ class MLP(nn.Module):
     def _forward(self, x: Tensor, residual: Optional[Tensor], chain_first: bool = False):
         if not isinstance(self.lins, nn.Sequential):
             return self.lins(x), False
+        if self.fused and x.is_cuda and not any(type(m) is BatchNorm for m in self.lins):
+            return self._forward_rows(x, residual)
         # same module sequence as the reference.  On device tensors a [Linear, BatchNorm, act] run is ONE autograd
         # node (GEMM + fused BatchNorm/activation kernels; the bias gradient falls out of the BatchNorm backward
         # pass) and a [BatchNorm, act] pair is one fused kernel pair; everything else is the stock module.
@@ -299,7 +306,44 @@ class MLP(nn.Module):
         return x, False
 
 
+    def _forward_rows(self, x: Tensor, residual: Optional[Tensor]):
+        """the `fused` form: (output, whether the residual is in it)"""
+        mods = list(self.lins)
+        i = 0
+        while i < len(mods):
+            lin, i = mods[i], i + 1
+            if not isinstance(lin, nn.Linear):                 # an activation behind an active dropout, the dropout itself
+                x = lin(x)
+                continue
+            norm = None
+            if i < len(mods) and type(mods[i]) in (LayerNorm, NoneNorm):
+                norm = mods[i].norm if type(mods[i]) is LayerNorm else None
+                i += 1
+            if i < len(mods) and isinstance(mods[i], nn.Dropout) and not (mods[i].training and mods[i].p > 0):
+                i += 1
+            act = _row_act(mods[i]) if i < len(mods) else None
+            if act is not None:
+                i += 1
+            x = _autocast_input(x)
+            res = residual if (residual is not None and i == len(mods) and residual.dtype == x.dtype
+                               and residual.shape == tuple(x.shape[:-1]) + (lin.out_features,)) else None
+            with torch.autocast("cuda", enabled=False):
+                if norm is None:
+                    x = _ops.linear_act(x, lin.weight, lin.bias, act or "none", residual=res)
+                else:
+                    x = _ops.linear_norm_act(x, lin.weight, lin.bias, norm.weight, norm.bias, norm.eps, act or "none", residual=res)
+            if res is not None:
+                return x, True
+        return x, False
+
+
 _ACT_NAMES = {nn.SiLU: "silu", nn.ReLU: "relu"}
+
+
+def _row_act(mod: nn.Module) -> Optional[str]:
+    if type(mod) is nn.ELU:
+        return "elu" if mod.alpha == 1.0 else None
+    return _ACT_NAMES.get(type(mod))
 
 
 def _autocast_input(x: Tensor) -> Tensor:
