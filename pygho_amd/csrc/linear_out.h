@@ -72,6 +72,7 @@ __global__ __launch_bounds__(kLoThreads) void linear_out_kernel(LsArgs a) {
   for (; blk < n_blocks; blk += stride) {
     asm volatile("" ::: "memory");                             // (see linear_stream.h)
     load_x(min(blk + stride, n_blocks - 1), xn);
+    __builtin_amdgcn_sched_barrier(0);                         // (loads first: see linear_tile.h)
     const int last = (int)min((int64_t)(MB * 16 - 1), m_rows - 1 - blk * (MB * 16));
     const char* rbase = reinterpret_cast<const char*>(a.r) + blk * (MB * 16) * a.r_ld * ES;
     char* obase = reinterpret_cast<char*>(a.out) + blk * (MB * 16) * N * (a.out_f32 ? 4 : ES);

@@ -242,6 +242,7 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_tile_kernel(LaArgs g) {
       __syncthreads();
       if constexpr (FULL) fetch(k_of(min(it + 1, n_it - 1)));   // (unconditional: the registers stay registers)
       else if (it + 1 < n_it) fetch(k_of(it + 1));
+      __builtin_amdgcn_sched_barrier(0);                         // (the scheduler puts the loads behind the products otherwise, and all of their latency in front of the next step)
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
         uint4 fm[NM];
@@ -278,34 +279,51 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_tile_kernel(LaArgs g) {
     } else {
       const T* res = reinterpret_cast<const T*>(g.res);
       T* out = reinterpret_cast<T*>(g.out);
+      // every load in front of the stores it does not depend on: a load's wait also waits for all older stores
+      float bias[NN][4];
+#pragma unroll
+      for (int j = 0; j < NN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int64_t n = n0 + wn + j * 16 + q * 4 + e;
+          bias[j][e] = n < g.n ? ro_param(g.bias, g.bias_dtype, n, 0.f) : 0.f;
+        }
 #pragma unroll
       for (int j = 0; j < NN; ++j) {
         const int64_t n = n0 + wn + j * 16 + q * 4;
         const int left = (int)min((int64_t)4, g.n - n);
-        if (left <= 0) continue;
-        float b4[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) b4[e] = e < left ? ro_param(g.bias, g.bias_dtype, n + e, 0.f) : 0.f;
+        for (int i = 0; i < NM; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] += bias[j][e];
+        if (g.z) {
+#pragma unroll
+          for (int i = 0; i < NM; ++i) {
+            const int64_t m = m0 + wm + i * 16 + r16;
+            const float u[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+            if (m < m_rows && left > 0) {
+              if (g.z_f32) la_store4<float>(reinterpret_cast<float*>(g.z) + m * g.n + n, left, g.z_vec, u);
+              else la_store4<T>(reinterpret_cast<T*>(g.z) + m * g.n + n, left, g.z_vec, u);
+            }
+          }
+        }
+        if (!out) continue;
+        float r[NM][4];
 #pragma unroll
         for (int i = 0; i < NM; ++i) {
           const int64_t m = m0 + wm + i * 16 + r16;
-          if (m >= m_rows) continue;
-          float u[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) u[e] = acc[i][j][e] + b4[e];
-          if (g.z) {
-            if (g.z_f32) la_store4<float>(reinterpret_cast<float*>(g.z) + m * g.n + n, left, g.z_vec, u);
-            else la_store4<T>(reinterpret_cast<T*>(g.z) + m * g.n + n, left, g.z_vec, u);
-          }
-          if (!out) continue;
+          for (int e = 0; e < 4; ++e) r[i][e] = 0.f;
+          if (res && m < m_rows && left > 0) la_load4<T>(res + m * g.res_ld + n, left, g.res_vec, r[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < NM; ++i) {
+          const int64_t m = m0 + wm + i * 16 + r16;
+          float u[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
           ro_act<P, 4>(u, g.act);
-          if (res) {
-            float r[4];
-            la_load4<T>(res + m * g.res_ld + n, left, g.res_vec, r);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) u[e] += r[e];
-          }
-          la_store4<T>(out + m * g.n + n, left, g.out_vec, u);
+          for (int e = 0; e < 4; ++e) u[e] += r[i][e];
+          if (m < m_rows && left > 0) la_store4<T>(out + m * g.n + n, left, g.out_vec, u);
         }
       }
     }
