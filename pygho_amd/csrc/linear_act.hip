@@ -37,19 +37,20 @@ static int la_param_check(const char* what, const void* p, int pdt, int dtype) {
   if (p && pdt != dtype && pdt != PYGHO_F32) { set_error("%s: parameters in the rows' type or in f32", what); return PYGHO_ERR_UNSUPPORTED; }
   return PYGHO_OK;
 }
-static int la_stride_check(const char* what, int64_t a, int64_t b, int dtype) {        // 32-bit offsets inside a block of 16 rows
-  if (a < 0 || b < 0 || std::max(a, b) * la_size(dtype) >= (1 << 28)) { set_error("%s: row strides of 0 .. 2^28 bytes", what); return PYGHO_ERR_UNSUPPORTED; }
+static int la_stride_check(const char* what, int64_t a, int64_t b, int dtype) {        // 32-bit offsets inside a block of 32 rows
+  if (a < 0 || b < 0 || std::max(a, b) * la_size(dtype) >= (1 << 27)) { set_error("%s: row strides of 0 .. 2^27 bytes", what); return PYGHO_ERR_UNSUPPORTED; }
   return PYGHO_OK;
 }
-static LaOperand la_operand(const void* p, int64_t ld, int dtype) { return LaOperand{p, ld, la_aligned(p, ld, la_size(dtype), 16) ? 1 : 0}; }
 
-// The form of a forward over (k, n).  W fits a CU's LDS: linear_stream.h where a norm needs the row, for narrow outputs (linear_out.h forms 64
-// channels at a time) and for k beyond what linear_out.h holds in registers; linear_out.h for the rest.  Otherwise tiles
+// The form of a forward over (k, n).  W fits a CU's LDS: linear_stream.h where a norm needs the row, for up to 128 output channels (linear_out.h forms
+// 64 at a time) and for k beyond what linear_out.h holds in registers; linear_out.h for the rest.  Otherwise tiles.
+// bf16, 1.05 M rows, silu, us of stream / out / tile: 128 -> 16 53 / 70 / 69, -> 32 65 / 75 / 102, -> 64 82 / 85 / 114, -> 128 111 / 121 / 315,
+// 256 -> 256 270 / 253 / 507
 enum { FORM_TILE = 0, FORM_STREAM = 1, FORM_OUT = 2 };
 static int la_form(int64_t k, int64_t n, int norm, int dtype) {
   return la_type(dtype, [&](auto ops) {
     const bool stream = ops.stream_lds(k, n, 0, false, false) <= kLsLds, out = !norm && ops.out_lds(k, n) <= kLsLds;
-    return stream && (!out || n <= 32) ? FORM_STREAM : out ? FORM_OUT : FORM_TILE;
+    return stream && (!out || n <= 128) ? FORM_STREAM : out ? FORM_OUT : FORM_TILE;
   });
 }
 static int la_forward(const LsArgs& a, int form, int norm, int dtype, hipStream_t st) {
@@ -60,7 +61,7 @@ static LsArgs la_stream_args(const void* x, int64_t x_ld, const void* w, int64_t
   const int es = la_size(dtype);
   LsArgs a{};
   a.x = x; a.x_ld = x_ld;
-  a.w = w; a.w_ld = w_ld; a.w_vec = la_aligned(w, w_ld, es, 16);
+  a.w = w; a.w_ld = w_ld;
   a.bias = bias; a.bias_dtype = bias_dtype; a.g = g; a.h = h; a.norm_dtype = norm_dtype;
   a.r = r; a.r_ld = r_ld;
   a.out = out;
@@ -72,13 +73,13 @@ static int la_tile_act(const void* x, int64_t x_ld, const void* w, int64_t w_ld,
                        void* y, void* z, int z_f32, int64_t m, int64_t k, int64_t n, int act, int dtype, hipStream_t st) {
   const int es = la_size(dtype);
   LaArgs a{};
-  a.a = la_operand(x, x_ld, dtype);
-  a.b = la_operand(w, w_ld, dtype);
+  a.a = {x, x_ld};
+  a.b = {w, w_ld};
   a.m = m; a.n = n; a.k = k;
-  a.out = y; a.out_vec = la_aligned(y, n, es, 4 * es);
-  a.z = z; a.z_f32 = z_f32; a.z_vec = la_aligned(z, n, z_f32 ? 4 : es, 4 * (z_f32 ? 4 : es));
+  a.out = y;
+  a.z = z; a.z_f32 = z_f32;
   a.bias = bias; a.bias_dtype = bias_dtype;
-  a.res = residual; a.res_ld = residual_ld; a.res_vec = la_aligned(residual, residual_ld, es, 4 * es);
+  a.res = residual; a.res_ld = residual_ld;
   a.act = act;
   return la_type(dtype, [&](auto ops) { return ops.tile_act(a, st); });
 }
@@ -92,7 +93,8 @@ static int64_t la_dw_slabs(int64_t m, int64_t k, int64_t n) {
 static int64_t la_pad4(int64_t v) { return (v + 3) / 4 * 4; }
 
 // The launches of a backward pass and its workspace, in bytes: [dz] [z] [slabs of the sums over n] [slabs of dW | db] [W^T]
-//   fused   dz, dX, dW and every sum from one streaming launch (operands aligned; its slabs are [sums | dW])
+//   fused   dz, dX, dW and every sum from one streaming launch (operands aligned; its slabs are [sums | dW]): 1.05 M rows of 128 -> 64 / 128 bf16
+//           151 / 220 us, in separate launches 261 / 357
 //   stream  dz with the sums (and dX where both copies of W fit) from a streaming launch
 //   else    dz by the row kernel from the pre-activation: kept by the forward, or (z) formed again in f32 where the forward streams
 struct LaSpace { int64_t dz, z, sums, dw, wt, total; int nsum; bool fused, stream, own_dz; };
@@ -236,8 +238,8 @@ extern "C" int pygho_linear_act_bwd(void* gx, void* gw, int gw_dtype, void* gb, 
   const bool db_here = gb && !sp.own_dz;                      // dz is gy itself: its column sums come with dW
   if (gw || db_here) {
     LaArgs a{};
-    a.a = la_operand(dz, dz_ld, dtype);
-    a.b = la_operand(x, x_ld, dtype);
+    a.a = {dz, dz_ld};
+    a.b = {x, x_ld};
     a.m = n; a.n = k; a.k = m_cap; a.k_dev = m_dev;
     a.slabs = reinterpret_cast<float*>(base + sp.dz + sp.z + sp.sums);
     a.slab_stride = la_pad4(n * k + n);

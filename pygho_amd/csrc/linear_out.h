@@ -31,7 +31,7 @@ __global__ __launch_bounds__(kLoThreads) void linear_out_kernel(LsArgs a) {
     for (int c = threadIdx.x; c < NP * KS * 4; c += blockDim.x) {
       const int n = c / (KS * 4), kc = c - n * (KS * 4);
       uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (n < N) v = ls_load16<T>(wp + (int64_t)n * a.w_ld, kc * E, K, a.w_vec);
+      if (n < N) v = ls_load16<T>(wp + (int64_t)n * a.w_ld, kc * E, K);
       *reinterpret_cast<uint4*>(lds_w + n * PITCH + kc * 16) = v;
     }
   } else {
@@ -40,7 +40,7 @@ __global__ __launch_bounds__(kLoThreads) void linear_out_kernel(LsArgs a) {
       const int k = c / cn, nc = c - k * cn;
       union { uint4 u; uint16_t h[8]; uint32_t f[4]; } v;
       v.u = make_uint4(0u, 0u, 0u, 0u);
-      if (k < K) v.u = ls_load16<T>(wp + (int64_t)k * a.w_ld, nc * E, N, a.w_vec);
+      if (k < K) v.u = ls_load16<T>(wp + (int64_t)k * a.w_ld, nc * E, N);
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         if constexpr (ES == 2) *reinterpret_cast<uint16_t*>(lds_w + (nc * E + j) * PITCH + k * 2) = v.h[j];
@@ -62,7 +62,7 @@ __global__ __launch_bounds__(kLoThreads) void linear_out_kernel(LsArgs a) {
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         if constexpr (XV) dst[mb][s] = s * (64 / ES) < K ? *reinterpret_cast<const uint4*>(base + off + s * 64) : make_uint4(0u, 0u, 0u, 0u);
-        else dst[mb][s] = ls_load16<T>(reinterpret_cast<const T*>(base + off), s * (64 / ES) + q * E, K, 0);
+        else dst[mb][s] = ls_load16<T>(reinterpret_cast<const T*>(base + off), s * (64 / ES) + q * E, K);
       }
     }
   };
@@ -109,7 +109,7 @@ __global__ __launch_bounds__(kLoThreads) void linear_out_kernel(LsArgs a) {
             for (int i = 0; i < 2; ++i) {
               const int nb = min(n0 + (t + i) * 16, NP - 16);
               if constexpr (NV) rv[mb][t + i] = *reinterpret_cast<const typename Raw4<T>::type*>(rbase + row + (nb + q * 4) * ES);
-              else rv[mb][t + i] = ls_load4<T>(reinterpret_cast<const T*>(rbase + row), nb + q * 4, N, 0);
+              else rv[mb][t + i] = ls_load4<T>(reinterpret_cast<const T*>(rbase + row), nb + q * 4, N);
             }
           }
         }
@@ -156,8 +156,8 @@ __global__ __launch_bounds__(kLoThreads) void linear_out_kernel(LsArgs a) {
           for (int i = 0; i < 2; ++i) {
             const int n = n0 + (t + i) * 16 + q * 4;
             if (rr <= last && (NV ? n0 + (t + i) * 16 : n) < N) {
-              if (a.out_f32) la_store4<float>(reinterpret_cast<float*>(obase + row32 + n * 4), NV ? 4 : N - n, NV, u[i]);
-              else la_store4<T>(reinterpret_cast<T*>(obase + row16 + n * ES), NV ? 4 : N - n, NV, u[i]);
+              if (a.out_f32) la_store4<float>(reinterpret_cast<float*>(obase + row32 + n * 4), NV ? 4 : N - n, u[i]);
+              else la_store4<T>(reinterpret_cast<T*>(obase + row16 + n * ES), NV ? 4 : N - n, u[i]);
             }
           }
         }

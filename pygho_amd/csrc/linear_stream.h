@@ -19,7 +19,7 @@ enum { LS_ACT = 0, LS_NORM = 1, LS_DACT = 2, LS_DNORM = 3 };
 
 struct LsArgs {
   const void* x; int64_t x_ld;
-  const void* w; int64_t w_ld; int w_vec; int w_trans;        // w_trans: w is stored [k][n] (the W of dz . W)
+  const void* w; int64_t w_ld; int w_trans;                   // w_trans: w is stored [k][n] (the W of dz . W)
   const void* bias; int bias_dtype; const void* g; const void* h; int norm_dtype;
   const void* r; int64_t r_ld;                                // residual (forward) / output gradient (backward)
   void* out; int out_f32;                                     // y / dz; out_f32 (LS_ACT): f32 values as they are
@@ -33,13 +33,11 @@ struct LsArgs {
 template <typename T> struct Raw4 { using type = uint2; };
 template <> struct Raw4<float> { using type = uint4; };
 
-// 16 bytes of a row from p (left elements remain): vectors where the operand's rows are aligned, element by element otherwise; zeros past the end
-template <typename T> __device__ __forceinline__ uint4 ls_load16(const T* row, int off, int end, int vec) {
+// 16 bytes of a row from element `off`; zeros from `end` on
+template <typename T> __device__ __forceinline__ uint4 ls_load16(const T* row, int off, int end) {
   constexpr int E = 16 / (int)sizeof(T);
   uint4 v = make_uint4(0u, 0u, 0u, 0u);
-  if (vec) {                                            // (aligned rows of whole vectors, or rows that reach beyond `end`)
-    if (off + E <= end) return *reinterpret_cast<const uint4*>(row + off);
-  }
+  if (off + E <= end) return la_ld<uint4>(row + off);
   if (off >= end) return v;
   const int left = end - off;
   uint32_t w[4];
@@ -55,9 +53,9 @@ template <typename T> __device__ __forceinline__ uint4 ls_load16(const T* row, i
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
-template <typename T> __device__ __forceinline__ typename Raw4<T>::type ls_load4(const T* row, int off, int end, int vec) {
+template <typename T> __device__ __forceinline__ typename Raw4<T>::type ls_load4(const T* row, int off, int end) {
   typename Raw4<T>::type v{};
-  if (vec && off + 4 <= end) return *reinterpret_cast<const typename Raw4<T>::type*>(row + off);
+  if (off + 4 <= end) return la_ld<typename Raw4<T>::type>(row + off);
   if (off >= end) return v;
   const int left = end - off;
   if constexpr (sizeof(T) == 4) {
@@ -130,8 +128,8 @@ template <int V, int S> __device__ __forceinline__ void ls_row_sums(float (&v)[V
 }
 
 // wavefronts per SIMD the registers are limited to (512 / this many per lane): latency, not throughput, is what a turn of 16 rows has most of
-// (fewer where they do not hold the kernel: the gradient through a norm of 65 .. 128 channels with the next block's rows in flight, and accesses
-// element by element with an address each)
+// (fewer where they do not hold the kernel: the gradient through a norm of 65 .. 128 channels with the next block's rows in flight, and masked accesses
+// with an address each)
 constexpr int ls_wps(int nb, int epi, int vec, int es) {
   if (vec != 3) return nb <= 2 ? 4 : nb == 4 ? 3 : nb == 8 ? 2 : 1;
   return nb <= 4 ? (nb == 4 && es == 4 && epi == LS_DNORM ? 3 : 4) : nb == 8 && epi != LS_DNORM ? 3 : 2;
@@ -156,7 +154,8 @@ constexpr int kLsDwWaves = 4;
 
 // VEC & 1: k is a whole number of 64-byte steps and x's rows allow 16-byte accesses.  VEC & 2: n is a whole number of 16 channels and the rows of r, out
 // and gx are on 16-byte boundaries (k of 16, with gx).  A block's rows then are one uniform base address, one 32-bit offset per lane and
-// constants -- 64-bit addresses per access, or masks per element, take more registers than the sums do.  Otherwise element by element.
+// constants -- 64-bit addresses per access, or masks per element, take more registers than the sums do.  Otherwise vectors from any element's
+// address with the ragged end masked (bf16 1.05 M rows of 100 -> 100: forward 160 us, 341 element by element; 128 -> 128 without a mask 111)
 //
 // DW (16-bit, k <= 128): the weight gradient in the same launch.  The workgroup's wavefronts go through their blocks in step; each puts its dz
 // and its x (16 rows, row-major) into LDS, and after a barrier forms its share of dW += dz^T x over the 64 rows, both operands read back
@@ -186,7 +185,7 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC, size
     for (int c = threadIdx.x; c < G::ROWS * cpr; c += blockDim.x) {
       const int n = c / cpr, kc = c - n * cpr;
       uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (n < N) v = ls_load16<T>(wp + (int64_t)n * a.w_ld, kc * E, K, a.w_vec);
+      if (n < N) v = ls_load16<T>(wp + (int64_t)n * a.w_ld, kc * E, K);
       *reinterpret_cast<uint4*>(lds_w + n * pitch + kc * 16) = v;
     }
   } else {
@@ -196,7 +195,7 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC, size
       const int k = c / CN, nc = c - k * CN;
       union { uint4 u; uint16_t h[8]; uint32_t f[4]; } v;
       v.u = make_uint4(0u, 0u, 0u, 0u);
-      if (k < K) v.u = ls_load16<T>(wp + (int64_t)k * a.w_ld, nc * E, N, a.w_vec);
+      if (k < K) v.u = ls_load16<T>(wp + (int64_t)k * a.w_ld, nc * E, N);
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         if constexpr (ES == 2) *reinterpret_cast<uint16_t*>(lds_w + (nc * E + j) * pitch + k * 2) = v.h[j];
@@ -210,7 +209,7 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC, size
       const int n = c / ck, kc = c - n * ck;
       union { uint4 u; uint32_t f[4]; } v;
       v.u = make_uint4(0u, 0u, 0u, 0u);
-      if (n < N) v.u = ls_load16<T>(wp + (int64_t)n * a.w_ld, kc * E, K, a.w_vec);
+      if (n < N) v.u = ls_load16<T>(wp + (int64_t)n * a.w_ld, kc * E, K);
 #pragma unroll
       for (int j = 0; j < E; ++j) *reinterpret_cast<uint32_t*>(lds_t + (kc * E + j) * G::PITCH_T + n * 4) = v.f[j];
     }
@@ -256,7 +255,7 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC, size
       if constexpr (XV) {
         if (kc * KC + s < KS) dst[s] = *reinterpret_cast<const uint4*>(base + off + s * 64);
       } else {
-        dst[s] = ls_load16<T>(reinterpret_cast<const T*>(base + off), s * (64 / ES) + q * E, K - kc * (KC * 64 / ES), 0);
+        dst[s] = ls_load16<T>(reinterpret_cast<const T*>(base + off), s * (64 / ES) + q * E, K - kc * (KC * 64 / ES));
       }
     }
   };
@@ -301,7 +300,7 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC, size
         if constexpr (NV) {
           if (nb * 16 < N_here) rv[nb] = *reinterpret_cast<const typename Raw4<T>::type*>(base + off + nb * 16 * ES);
         } else {
-          rv[nb] = ls_load4<T>(reinterpret_cast<const T*>(base + off), nb * 16 + q * 4, N, 0);
+          rv[nb] = ls_load4<T>(reinterpret_cast<const T*>(base + off), nb * 16 + q * 4, N);
         }
       }
     }
@@ -411,7 +410,7 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC, size
 #pragma unroll
           for (int i = 0; i < 2 && nb + i < NB; ++i) {
             const int n = (nb + i) * 16 + q * 4;
-            if (row_ok && (NV ? (nb + i) * 16 : n) < N_here) la_store4<O>(reinterpret_cast<O*>(base + row + n * sizeof(O)), NV ? 4 : N - n, NV, val[nb + i]);
+            if (row_ok && (NV ? (nb + i) * 16 : n) < N_here) la_store4<O>(reinterpret_cast<O*>(base + row + n * sizeof(O)), NV ? 4 : N - n, val[nb + i]);
           }
         }
       };
@@ -575,7 +574,7 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC, size
               for (int i = 0; i < 2; ++i) {
                 const int k = (kg + t + i) * 16 + q * 4;
                 const float o4[4] = {o[t + i][0], o[t + i][1], o[t + i][2], o[t + i][3]};
-                if (row_ok && k < K) la_store4<T>(reinterpret_cast<T*>(base + row + k * ES), NV ? 4 : K - k, NV, o4);
+                if (row_ok && k < K) la_store4<T>(reinterpret_cast<T*>(base + row + k * ES), NV ? 4 : K - k, o4);
               }
             }
           }

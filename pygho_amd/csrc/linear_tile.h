@@ -21,20 +21,26 @@ enum { LA_ROWS = 0, LA_COLS = 1 };
 // epilogues: bias, activation, residual, one store (the pre-activation beside it if asked); f32 slab of a split product
 enum { LA_ACT = 0, LA_SLAB = 4 };
 
-struct LaOperand { const void* p; int64_t ld; int vec; };      // vec: rows on 16-byte boundaries (16-byte loads where they fit)
+struct LaOperand { const void* p; int64_t ld; };
 
 struct LaArgs {
   LaOperand a, b;                     // P (m, k), Q (n, k)
   int64_t m; int64_t n; int64_t k;    // k: of the whole product; LA_SLAB: an upper bound of it (k_dev: the true one)
   const int32_t* k_dev;
-  void* out; int out_vec;             // nullable: only z
-  void* z; int z_f32; int z_vec;      // nullable: the pre-activation, in the storage type or in f32
+  void* out;                          // nullable: only z
+  void* z; int z_f32;                 // nullable: the pre-activation, in the storage type or in f32
   const void* bias; int bias_dtype;
-  const void* res; int64_t res_ld; int res_vec;
+  const void* res; int64_t res_ld;
   int act;
   float* slabs; int64_t slab_stride; int splits;      // LA_SLAB: slab s = [m * n product | m column sums (want_sums)]
   int want_sums;
 };
+
+// 16 or 8 bytes at any element's address.  gfx950 loads and stores vectors from there in one instruction (a packed type makes the compiler use it),
+// so odd widths and strides need no path of their own: what is left is the ragged end of a row
+template <typename V, typename T> struct __attribute__((packed, aligned(sizeof(T)))) LaAny { uint32_t w[sizeof(V) / 4]; };
+template <typename V, typename T> __device__ __forceinline__ V la_ld(const T* p) { return __builtin_bit_cast(V, *reinterpret_cast<const LaAny<V, T>*>(p)); }
+template <typename V, typename T> __device__ __forceinline__ void la_st(T* p, const V& v) { *reinterpret_cast<LaAny<V, T>*>(p) = __builtin_bit_cast(LaAny<V, T>, v); }
 
 // one step of k (64 bytes per row): bf16 / f16 one 16x16x32 MFMA, f32 four 16x16x4 (element j of every lane's 4 is k = 4 q + j on both sides)
 template <typename T> __device__ __forceinline__ la_f32x4_t la_mfma(const uint4& a, const uint4& b, la_f32x4_t c) {
@@ -86,7 +92,7 @@ template <typename T, int MODE, int R, int THREADS> struct LaTile {
     const int64_t inner = (MODE == LA_ROWS ? k0 : r0) + lc * E, inner_end = MODE == LA_ROWS ? k_end : n_rows;
     if (outer >= outer_end || inner >= inner_end) return v;
     const T* p = base + outer * op.ld + inner;
-    if (op.vec && inner + E <= inner_end) return *reinterpret_cast<const uint4*>(p);
+    if (inner + E <= inner_end) return la_ld<uint4>(p);
     const int left = (int)min((int64_t)E, inner_end - inner);
     uint32_t w[4];
 #pragma unroll
@@ -101,13 +107,13 @@ template <typename T, int MODE, int R, int THREADS> struct LaTile {
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
-  // aligned rows and whole steps of k (FULL): one uniform base and 32-bit offsets; a row past the end repeats the last one (its products are not stored)
+  // whole steps of k (FULL): one uniform base and 32-bit offsets; a row past the end repeats the last one (its products are not stored)
   static __device__ __forceinline__ uint4 load_full(const LaOperand& op, int64_t r0, int64_t n_rows, int64_t k0, int i) {
     static_assert(MODE == LA_ROWS && CHUNKS % THREADS == 0, "row operands");
     const char* base = reinterpret_cast<const char*>(op.p) + (r0 * op.ld + k0) * ES;
     const int last = (int)min((int64_t)(R - 1), n_rows - 1 - r0);
-    return *reinterpret_cast<const uint4*>(base + (uint32_t)min(i * (THREADS / 8) + (int)threadIdx.x / 8, last) * (uint32_t)(op.ld * ES) +
-                                           ((int)threadIdx.x % 8) * 16);
+    return la_ld<uint4>(reinterpret_cast<const T*>(base + (uint32_t)min(i * (THREADS / 8) + (int)threadIdx.x / 8, last) * (uint32_t)(op.ld * ES) +
+                                                   ((int)threadIdx.x % 8) * 16));
   }
   static __device__ __forceinline__ void store(char* lds, const uint4& v, int i) {
     const int c = i * THREADS + (int)threadIdx.x;
@@ -133,14 +139,14 @@ template <typename T, int MODE, int R, int THREADS> struct LaTile {
 
 constexpr int kLaChunk = 128;         // rows of a split product's reduction per chunk: chunk j belongs to split j % splits
 
-// 4 consecutive elements (of row m, from n) <-> registers; `vec`: the rows are aligned for one access of 4 elements
-template <typename T> __device__ __forceinline__ void la_load4(const T* p, int left, int vec, float (&v)[4]) {
-  if (vec && left >= 4) {
+// 4 consecutive elements (of row m, from n) <-> registers, `left` of them in the row
+template <typename T> __device__ __forceinline__ void la_load4(const T* p, int left, float (&v)[4]) {
+  if (left >= 4) {
     if constexpr (sizeof(T) == 4) {
-      const uint4 r = *reinterpret_cast<const uint4*>(p);
+      const uint4 r = la_ld<uint4>(p);
       v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
     } else {
-      const uint2 r = *reinterpret_cast<const uint2*>(p);
+      const uint2 r = la_ld<uint2>(p);
       float t[8];
       Vec16<T>::unpack(make_uint4(r.x, r.y, 0u, 0u), t);
 #pragma unroll
@@ -151,14 +157,14 @@ template <typename T> __device__ __forceinline__ void la_load4(const T* p, int l
     for (int i = 0; i < 4; ++i) v[i] = i < left ? load_as_acc<T>(p + i) : 0.f;
   }
 }
-template <typename T> __device__ __forceinline__ void la_store4(T* p, int left, int vec, const float (&v)[4]) {
-  if (vec && left >= 4) {
+template <typename T> __device__ __forceinline__ void la_store4(T* p, int left, const float (&v)[4]) {
+  if (left >= 4) {
     if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<uint4*>(p) = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+      la_st(p, make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])));
     } else {
       const float t[8] = {v[0], v[1], v[2], v[3], 0.f, 0.f, 0.f, 0.f};
       const uint4 r = Vec16<T>::pack(t);
-      *reinterpret_cast<uint2*>(p) = make_uint2(r.x, r.y);
+      la_st(p, make_uint2(r.x, r.y));
     }
   } else {
 #pragma unroll
@@ -302,8 +308,8 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_tile_kernel(LaArgs g) {
             const int64_t m = m0 + wm + i * 16 + r16;
             const float u[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
             if (m < m_rows && left > 0) {
-              if (g.z_f32) la_store4<float>(reinterpret_cast<float*>(g.z) + m * g.n + n, left, g.z_vec, u);
-              else la_store4<T>(reinterpret_cast<T*>(g.z) + m * g.n + n, left, g.z_vec, u);
+              if (g.z_f32) la_store4<float>(reinterpret_cast<float*>(g.z) + m * g.n + n, left, u);
+              else la_store4<T>(reinterpret_cast<T*>(g.z) + m * g.n + n, left, u);
             }
           }
         }
@@ -314,7 +320,7 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_tile_kernel(LaArgs g) {
           const int64_t m = m0 + wm + i * 16 + r16;
 #pragma unroll
           for (int e = 0; e < 4; ++e) r[i][e] = 0.f;
-          if (res && m < m_rows && left > 0) la_load4<T>(res + m * g.res_ld + n, left, g.res_vec, r[i]);
+          if (res && m < m_rows && left > 0) la_load4<T>(res + m * g.res_ld + n, left, r[i]);
         }
 #pragma unroll
         for (int i = 0; i < NM; ++i) {
@@ -323,7 +329,7 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_tile_kernel(LaArgs g) {
           ro_act<P, 4>(u, g.act);
 #pragma unroll
           for (int e = 0; e < 4; ++e) u[e] += r[i][e];
-          if (m < m_rows && left > 0) la_store4<T>(out + m * g.n + n, left, g.out_vec, u);
+          if (m < m_rows && left > 0) la_store4<T>(out + m * g.n + n, left, u);
         }
       }
     }
@@ -363,7 +369,10 @@ template <typename T, int MA, int MB, int EPI> static int la_any(const LaArgs& a
   if (a.n <= 16) return la_go<T, MA, MB, 64, 16, 4, 1, EPI>(a, kLaGrid, st);
   // 16-bit products large enough for a 256 x 256 tile per CU: a wavefront's 128 x 64 part reads 12 fragments of LDS per 32 MFMAs, a 64 x 64 part 8 per 16
   if constexpr (sizeof(T) == 2 && EPI == LA_ACT)
-    if (a.n > 128 && count(256, 256) >= 256 && a.a.vec && a.b.vec && a.k % 64 == 0) return la_go<T, MA, MB, 256, 256, 2, 4, EPI, true>(a, kLaGrid, st);
+    // (bf16 forward 65536 x 512 -> 512 72 us, 138 with 128 x 128 tiles; 262144 x 512 -> 256 170, 278).  Its 32-bit offsets reach over 256 rows.  The weight gradient stays on 128 x 128
+    // tiles with a condition per load: unconditional ones took registers and a workgroup per CU with them (84 -> 116 us)
+    if (a.n > 128 && count(256, 256) >= 256 && a.k % 64 == 0 && std::max(a.a.ld, a.b.ld) * (int64_t)sizeof(T) < (1 << 24))
+      return la_go<T, MA, MB, 256, 256, 2, 4, EPI, true>(a, kLaGrid, st);
   if (a.n > 64 && a.m > 64 && count(128, 128) >= 256) return la_go<T, MA, MB, 128, 128, 2, 2, EPI>(a, kLaGrid, st);
   return la_go<T, MA, MB, 64, 64, 2, 2, EPI>(a, kLaGrid, st);
 }

@@ -42,6 +42,7 @@ def test_linear_refusals(lib):
     assert fwd(y=None) == 1 and fwd(x=None) == 1 and fwd(w=None) == 1 and b"null" in lib.pygho_last_error()
     assert fwd(dt=F64) == 2 and fwd(bias=ONE, bdt=F16) == 2
     assert fwd(x_ld=-1) == 2 and fwd(x_ld=1 << 28) == 2 and fwd(r=ONE, r_ld=1 << 27) == 2 and b"strides" in lib.pygho_last_error()
+    assert fwd(x_ld=1 << 26) == 2 and fwd(r=ONE, r_ld=1 << 26) == 2      # 32 rows of 2^27 bytes pass a 32-bit offset
     # a norm over more channels than a workgroup holds needs the pre-activation's buffer
     assert lib.pygho_linear_act_keeps(512, 512, 1, 2, BF16) == 2 and fwd(z=None, norm=1, k=512, n=512) == 1 and b"keeps" in lib.pygho_last_error()
     assert lib.pygho_linear_act_keeps(512, 512, 0, 2, BF16) == 1 and lib.pygho_linear_act_keeps(512, 512, 0, 0, BF16) == 0
