@@ -101,16 +101,17 @@ struct LaSpace { int64_t dz, z, sums, dw, wt, total; int nsum; bool fused, strea
 static LaSpace la_space(int64_t m, int64_t k, int64_t n, int norm, int act, int dtype, bool aligned) {
   LaSpace s{};
   s.nsum = norm ? 3 : 1;
+  const int64_t slabs = std::min<int64_t>(kLsGrid, ceil_div(m, 16));      // a streaming launch: at most one workgroup per block of rows
   s.fused = aligned && la_type(dtype, [&](auto ops) { return ops.dw_fits(k, n, s.nsum); });
   if (s.fused) {
-    s.total = s.dw = kLsGrid * la_pad4(s.nsum * n + n * k) * 4;
+    s.total = s.dw = slabs * la_pad4(s.nsum * n + n * k) * 4;
     return s;
   }
   s.own_dz = norm || act != kActNone;
   s.stream = s.own_dz && n <= ls_bwd_max(norm, la_size(dtype)) && la_type(dtype, [&](auto ops) { return ops.stream_lds(k, n, s.nsum, false, false) <= kLsLds; });
   s.dz = s.own_dz ? (m * n * la_size(dtype) + 15) / 16 * 16 : 0;
   s.z = s.own_dz && !s.stream && la_form(k, n, norm, dtype) != FORM_TILE ? (m * n * 4 + 15) / 16 * 16 : 0;
-  s.sums = !s.own_dz ? 0 : s.stream ? kLsGrid * la_pad4(s.nsum * n) * 4 : ln_bwd_slab_floats(m, n, s.nsum) * 4;
+  s.sums = !s.own_dz ? 0 : s.stream ? slabs * la_pad4(s.nsum * n) * 4 : ln_bwd_slab_floats(m, n, s.nsum) * 4;
   s.dw = la_dw_slabs(m, k, n) * la_pad4(n * k + n) * 4;
   s.wt = la_form(n, k, 0, dtype) == FORM_TILE ? (n * k * la_size(dtype) + 15) / 16 * 16 : 0;
   s.total = s.dz + s.z + s.sums + s.dw + s.wt;
