@@ -9,6 +9,9 @@
 // gg / gh: a lane keeps its channels' sums over all rows of its workgroup; workgroups write one slab each, a second launch adds the
 // slabs in a fixed order.  Chunk k of the rows belongs to workgroup k % grid, so a slab depends on the true rows only: a launch sized for a
 // capacity (m_dev: the count is on the device) gives the bits of an exactly sized one.
+// Measured: bf16 1.83 M x 128 with residual 287 us forward (1.41 GB: 4.9 TB/s), 327 us backward (1.41 GB: 4.3 TB/s) + fold 6; f16 40531 x 1000
+// forward 52 us (0.24 GB: 4.7 TB/s); f32 23719 x 193 (element by element) 14 + 18 + 5 us; f32 128 x 128 forward 4.8 us.
+// 16-byte vectors where rows allow them, single elements otherwise: neighbouring lanes then still read neighbouring addresses
 #include "row_ops.h"
 
 namespace pygho {

@@ -70,12 +70,12 @@ static LsArgs la_stream_args(const void* x, int64_t x_ld, const void* w, int64_t
   return a;
 }
 static int la_tile_act(const void* x, int64_t x_ld, const void* w, int64_t w_ld, const void* bias, int bias_dtype, const void* residual, int64_t residual_ld,
-                       void* y, void* z, int z_f32, int64_t m, int64_t k, int64_t n, int act, int dtype, hipStream_t st) {
+                       void* y, void* z, int z_f32, int64_t m, const int32_t* m_dev, int64_t k, int64_t n, int act, int dtype, hipStream_t st) {
   const int es = la_size(dtype);
   LaArgs a{};
   a.a = {x, x_ld};
   a.b = {w, w_ld};
-  a.m = m; a.n = n; a.k = k;
+  a.m = m; a.n = n; a.k = k; a.dev = m_dev;
   a.out = y;
   a.z = z; a.z_f32 = z_f32;
   a.bias = bias; a.bias_dtype = bias_dtype;
@@ -141,9 +141,9 @@ extern "C" int pygho_linear_act(void* y, void* z, const void* x, int64_t x_ld, c
   hipStream_t st = (hipStream_t)stream;
   if (const int form = la_form(k, n, norm, dtype); form != FORM_TILE)
     return la_forward(la_stream_args(x, x_ld, w, w_ld, bias, bias_dtype, g, h, norm_dtype, residual, residual_ld, y, m, k, n, eps, act, dtype), form, norm, dtype, st);
-  if (!norm) return la_tile_act(x, x_ld, w, w_ld, bias, bias_dtype, residual, residual_ld, y, z, 0, m, k, n, act, dtype, st);
+  if (!norm) return la_tile_act(x, x_ld, w, w_ld, bias, bias_dtype, residual, residual_ld, y, z, 0, m, nullptr, k, n, act, dtype, st);
   if (!z) { set_error("linear_act: this norm needs the pre-activation's buffer (pygho_linear_act_keeps)"); return PYGHO_ERR_INVALID; }
-  if (int rc = la_tile_act(x, x_ld, w, w_ld, bias, bias_dtype, nullptr, 0, nullptr, z, 1, m, k, n, kActNone, dtype, st)) return rc;
+  if (int rc = la_tile_act(x, x_ld, w, w_ld, bias, bias_dtype, nullptr, 0, nullptr, z, 1, m, nullptr, k, n, kActNone, dtype, st)) return rc;
   return ln_fwd_launch(y, z, n, g, h, norm_dtype, residual, residual_ld, m, n, (float)eps, act, dtype, PYGHO_F32, st);
 }
 
@@ -210,6 +210,7 @@ extern "C" int pygho_linear_act_bwd(void* gx, void* gw, int gw_dtype, void* gb, 
       if (sp.z) {
         LsArgs a = la_stream_args(x, x_ld, w, w_ld, bias, bias_dtype, nullptr, nullptr, 0, nullptr, 0, base + sp.dz, m_cap, k, n, 0.0, kActNone, dtype);
         a.out_f32 = 1;
+        a.m_dev = m_dev;
         if (int rc = la_forward(a, la_form(k, n, 0, dtype), 0, dtype, st)) return rc;
         z = base + sp.dz;
       }
@@ -229,11 +230,12 @@ extern "C" int pygho_linear_act_bwd(void* gx, void* gw, int gw_dtype, void* gb, 
     if (const int form = la_form(n, k, 0, dtype); form != FORM_TILE) {
       LsArgs a = la_stream_args(dz, dz_ld, w, w_ld, nullptr, 0, nullptr, nullptr, 0, nullptr, 0, gx, m_cap, n, k, 0.0, kActNone, dtype);
       a.w_trans = 1;
+      a.m_dev = m_dev;
       if (int rc = la_forward(a, form, 0, dtype, st)) return rc;
     } else {
       void* wt = base + sp.dz + sp.z + sp.sums + sp.dw;
       if (int rc = la_type(dtype, [&](auto ops) { return ops.transpose(wt, w, w_ld, n, k, st); })) return rc;
-      if (int rc = la_tile_act(dz, dz_ld, wt, n, nullptr, 0, nullptr, 0, gx, nullptr, 0, m_cap, n, k, kActNone, dtype, st)) return rc;
+      if (int rc = la_tile_act(dz, dz_ld, wt, n, nullptr, 0, nullptr, 0, gx, nullptr, 0, m_cap, m_dev, n, k, kActNone, dtype, st)) return rc;
     }
   }
   const bool db_here = gb && !sp.own_dz;                      // dz is gy itself: its column sums come with dW
@@ -241,7 +243,7 @@ extern "C" int pygho_linear_act_bwd(void* gx, void* gw, int gw_dtype, void* gb, 
     LaArgs a{};
     a.a = {dz, dz_ld};
     a.b = {x, x_ld};
-    a.m = n; a.n = k; a.k = m_cap; a.k_dev = m_dev;
+    a.m = n; a.n = k; a.k = m_cap; a.dev = m_dev;
     a.slabs = reinterpret_cast<float*>(base + sp.dz + sp.z + sp.sums);
     a.slab_stride = la_pad4(n * k + n);
     a.splits = (int)la_dw_slabs(m_cap, k, n);

@@ -3,7 +3,7 @@
 // As linear_stream.h: W in LDS for the whole launch, wavefronts walk blocks of rows without barriers.  Here the roles of the registers are the other
 // way round: a block's x (32 rows x K) stays in them while the output channels go by, 64 at a time -- no state per output channel, so the width is
 // bounded by LDS only, and every fragment of W serves 32 rows (at K = N = 256 with 16 rows per fragment, reading W took 64 of the ~114 cycles that
-// HBM takes per row, and the launch 0.73 ms instead of the 0.46 ms of its bytes).
+// HBM takes per row, and the launch 0.73 ms instead of the 0.46 ms of its bytes).  Measured: bf16 2.39 M x 256 -> 256 0.51 ms = 4.8 TB/s.
 #pragma once
 #include "linear_stream.h"
 
@@ -52,7 +52,7 @@ __global__ __launch_bounds__(kLoThreads) void linear_out_kernel(LsArgs a) {
   __syncthreads();
 
   const int waves = blockDim.x >> 6;
-  const int64_t m_rows = a.m, n_blocks = (m_rows + MB * 16 - 1) / (MB * 16), stride = (int64_t)gridDim.x * waves;
+  const int64_t m_rows = a.m_dev ? *a.m_dev : a.m, n_blocks = (m_rows + MB * 16 - 1) / (MB * 16), stride = (int64_t)gridDim.x * waves;
   auto load_x = [&](int64_t b, uint4 (&dst)[MB][KS]) {
     const int last = (int)min((int64_t)(MB * 16 - 1), m_rows - 1 - b * (MB * 16));
     const char* base = reinterpret_cast<const char*>(a.x) + b * (MB * 16) * a.x_ld * ES;

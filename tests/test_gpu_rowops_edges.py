@@ -138,6 +138,61 @@ def test_rows_at_odd_addresses(dev, dtype, k, n):
         assert torch.equal(g, v.to(dtype)), g.shape
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("k,n", [(128, 128), (384, 128), (100, 36), (256, 256), (100, 513), (512, 512), (300, 20)])
+@pytest.mark.parametrize("true", [0, 1, 300])
+def test_rows_behind_the_device_count_stay_as_they_were(dev, dtype, k, n, true):
+    """the C entry with a capacity of 500 rows and the true count on the device: gx behind the count keeps its bytes, what x, gy and z hold
+    there (NaN) reaches nothing"""
+    from pygho_amd import _ops
+    from pygho_amd._native import DTYPE_CODE, check, lib, ptr, stream_ptr
+    gen = torch.Generator(device=dev)
+    gen.manual_seed(k + n + true)
+    cap, code, act = 500, DTYPE_CODE[dtype], _ops.ROW_ACT_CODE["relu"]
+    x, w, b, gy = (integers(gen, s, dev, most, dtype) for s, most in (((cap, k), 2), ((n, k), 2), ((n,), 9), ((cap, n), 2)))
+    _, gx, gw, gb = exact(x[:true], w, b, gy[:true])
+    keeps = int(lib().pygho_linear_act_keeps(k, n, 0, act, code))
+    z = (x.double() @ w.double().t() + b.double()).to(dtype) if keeps else None
+    for t in (x, gy) + ((z,) if keeps else ()):
+        t[true:] = float("nan")
+    out, gw2, gb2 = torch.full((cap, k), 77.0, dtype=dtype, device=dev), torch.empty_like(w), torch.empty_like(b)
+    count = torch.tensor([true], dtype=torch.int32, device=dev)
+    nbytes = int(lib().pygho_linear_act_bwd_workspace(cap, k, n, 0, act, code))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    check(lib().pygho_linear_act_bwd(ptr(out), ptr(gw2), code, ptr(gb2), code, None, 0, None, 0, ptr(z), ptr(x), k, ptr(w), k, ptr(b), code, 0, None, None,
+                                     0, 0.0, ptr(gy), n, cap, ptr(count), k, n, act, code, ptr(ws), nbytes, stream_ptr(dev)), "linear_act_bwd")
+    assert bool((out[true:] == 77.0).all())
+    assert torch.equal(out[:true], gx.to(dtype)) and torch.equal(gw2, gw.to(dtype)) and torch.equal(gb2, gb.to(dtype))
+
+
+@pytest.mark.parametrize("k,n", [(128, 128), (256, 130), (520, 130)])
+def test_more_elements_than_32_bits_count(dev, k, n):
+    """the last rows of 2^31 elements and 2^32 bytes give the bits that they give alone; parameters' gradients of gy that is zero elsewhere too"""
+    from pygho_amd import _ops
+    gen = torch.Generator(device=dev)
+    gen.manual_seed(k)
+    m, tail = (1 << 31) // min(k, n) + 100001, 777
+    w, b, xt, gt = (integers(gen, s, dev, 2, torch.bfloat16) for s in ((n, k), (n,), (tail, k), (tail, n)))
+    x = torch.ones(m, k, dtype=torch.bfloat16, device=dev)
+    gy = torch.zeros(m, n, dtype=torch.bfloat16, device=dev)
+    x[m - tail:], gy[m - tail:] = xt, gt
+    y, gx, gw, gb = exact(xt, w, b, gt)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    out = _ops.linear_act(*leaves, act="relu")
+    assert torch.equal(out.detach()[m - tail:], y.to(torch.bfloat16))
+    grads = torch.autograd.grad(out, leaves, gy)
+    assert torch.equal(grads[0][m - tail:], gx.to(torch.bfloat16)) and not grads[0][: m - tail].any()
+    assert torch.equal(grads[1], gw.to(torch.bfloat16)) and torch.equal(grads[2], gb.to(torch.bfloat16))
+    del out, grads
+    if k == 128:
+        ln = _ops.layer_norm_act(x.detach(), act="silu")
+        assert torch.equal(ln[m - tail:], _ops.layer_norm_act(xt, act="silu"))
+        del ln
+        a, = torch.autograd.grad(_ops.layer_norm_act(x, act="elu"), x, gy)
+        c, = torch.autograd.grad(_ops.layer_norm_act(xt.requires_grad_(True), act="elu"), xt, gt)
+        assert torch.equal(a[m - tail:], c)
+
+
 def test_small_calls_take_small_workspaces(dev):
     from pygho_amd._native import DTYPE_CODE, lib
     at = [int(lib().pygho_linear_act_bwd_workspace(m, 128, 128, 1, 2, DTYPE_CODE[torch.bfloat16])) for m in (1, 16, 100, 10 ** 5, 10 ** 7)]
