@@ -42,6 +42,15 @@ from typing import Any, Callable, Iterable
 import torch
 
 
+def _capture_mode() -> str:
+    """how strictly a capture treats the process's OTHER threads.  With an RCCL process group there is one that the program does not control:
+    torch's watchdog polls the events of finished collectives until it has dropped them from its list, a query that a capture in the default
+    mode ("global") refuses -- the watchdog then ends the process ("operation not permitted when stream is capturing").  Queries of another
+    thread touch nothing that is being captured, so with such a group only the capturing thread is held to the rules."""
+    import torch.distributed as dist
+    return "thread_local" if dist.is_available() and dist.is_initialized() and "nccl" in str(dist.get_backend()) else "global"
+
+
 class GraphedStep:
     """``GraphedStep(fn)`` warms ``fn`` up on a side stream, captures one call into a HIP graph and replays it."""
 
@@ -55,7 +64,7 @@ class GraphedStep:
                 fn()
         torch.cuda.current_stream().wait_stream(side)
         self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
+        with torch.cuda.graph(self.graph, capture_error_mode=_capture_mode()):
             self.output = fn()
 
     def replay(self) -> Any:
@@ -124,7 +133,7 @@ class SlotStep:
         slot.reset_caches()
         calls0 = sync.allreduce_calls if sync is not None else 0
         self.graph = torch.cuda.CUDAGraph()
-        with slot.rows(), torch.cuda.graph(self.graph):
+        with slot.rows(), torch.cuda.graph(self.graph, capture_error_mode=_capture_mode()):
             slot.launch()
             self.output = step_fn(dd)
         self._calls_per_step = (sync.allreduce_calls - calls0) if sync is not None else 0     # collectives inside ONE captured step
