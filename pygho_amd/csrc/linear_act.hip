@@ -44,8 +44,8 @@ static int la_stride_check(const char* what, int64_t a, int64_t b, int dtype) { 
 
 // The form of a forward over (k, n).  W fits a CU's LDS: linear_stream.h where a norm needs the row, for up to 128 output channels (linear_out.h forms
 // 64 at a time) and for k beyond what linear_out.h holds in registers; linear_out.h for the rest.  Otherwise tiles.
-// bf16, 1.05 M rows, silu, us of stream / out / tile: 128 -> 16 53 / 70 / 69, -> 32 65 / 75 / 102, -> 64 82 / 85 / 114, -> 128 111 / 121 / 315,
-// 256 -> 256 270 / 253 / 507
+// bf16, 1.05 M rows, silu, us of stream / out / tile: 128 -> 16 53 / 70 / 68, -> 32 65 / 75 / 88, -> 64 82 / 85 / 108, -> 128 111 / 121 / 183,
+// 256 -> 256 270 / 253 / 436
 enum { FORM_TILE = 0, FORM_STREAM = 1, FORM_OUT = 2 };
 static int la_form(int64_t k, int64_t n, int norm, int dtype) {
   return la_type(dtype, [&](auto ops) {

@@ -7,7 +7,7 @@
 // Column operands stay in their storage order in LDS; 16-bit fragments are read back transposed by the LDS itself (ds_read_b64_tr_b16),
 // f32 ones element by element (conflict-free, and an f32 MFMA takes 32 cycles).
 // f32 products run on v_mfma_f32_16x16x4f32: true f32, no reduced-precision path.
-// Measured, bf16 65536 x 512 -> 512: forward 72 us without, 87 with the f32 pre-activation stored (34 GFLOP: 470 / 390 TFLOP/s, bound by the wait for a
+// Measured, bf16 65536 x 512 -> 512: forward 66 us with a 16-bit pre-activation stored, 87 with an f32 one (34 GFLOP: 520 / 390 TFLOP/s, bound by the wait for a
 // step's loads at one workgroup per CU), weight gradient 85 us (400 TFLOP/s)
 #pragma once
 #include "row_ops.h"
@@ -174,9 +174,10 @@ template <typename T> __device__ __forceinline__ void la_store4(T* p, int left, 
   }
 }
 
-// a workgroup of WM x WN wavefronts forms BM x BN output tiles
+// a workgroup of WM x WN wavefronts forms BM x BN output tiles.  Two wavefronts per SIMD at least: left alone, the 128 x 128 tile took 259 registers
+// and had one (bf16 forward 65536 x 500 -> 500 163 us, with two 92 .. 103)
 template <typename T, int MA, int MB, int BM, int BN, int WM, int WN, int EPI, bool FULL = false>
-__global__ __launch_bounds__(WM * WN * 64) void linear_tile_kernel(LaArgs g) {
+__global__ __launch_bounds__(WM * WN * 64, 2) void linear_tile_kernel(LaArgs g) {
   using TA = LaTile<T, MA, BM, WM * WN * 64>;
   using TB = LaTile<T, MB, BN, WM * WN * 64>;
   constexpr int KE = TA::KE, TM = BM / WM, TN = BN / WN, NM = TM / 16, NN = TN / 16;
@@ -363,14 +364,15 @@ template <typename T, int MA, int MB, int BM, int BN, int WM, int WN, int EPI, b
 
 constexpr int kLaGrid = 1 << 20;        // workgroups of a launch (a larger product loops)
 
-// Tile of an (m, n) product without a norm: the largest that still gives every CU a workgroup, no wider than the product
+// Tile of an (m, n) product without a norm: the largest that still gives every CU a workgroup, no wider than the product (128 x 128 against 64 x 64, bf16:
+// 65536 x 500 -> 500 forward 92 us, 100, gradients 445, 502; gradients of 1.05 M x 256 -> 256 970, 1276)
 template <typename T, int MA, int MB, int EPI> static int la_any(const LaArgs& a, hipStream_t st) {
   const int64_t sp = EPI == LA_SLAB ? a.splits : 1;
   auto count = [&](int bm, int bn) { return ceil_div(a.m, bm) * ceil_div(a.n, bn) * sp; };
   if (a.n <= 16) return la_go<T, MA, MB, 64, 16, 4, 1, EPI>(a, kLaGrid, st);
   // 16-bit products large enough for a 256 x 256 tile per CU: a wavefront's 128 x 64 part reads 12 fragments of LDS per 32 MFMAs, a 64 x 64 part 8 per 16
   if constexpr (sizeof(T) == 2 && EPI == LA_ACT)
-    // (bf16 forward 65536 x 512 -> 512 72 us, 138 with 128 x 128 tiles; 262144 x 512 -> 256 170, 278).  Its 32-bit offsets reach over 256 rows.  The weight gradient stays on 128 x 128
+    // (bf16 forward 65536 x 512 -> 512 66 us, 80 with 128 x 128 tiles; 262144 x 512 -> 256 151, 168).  Its 32-bit offsets reach over 256 rows.  The weight gradient stays on 128 x 128
     // tiles with a condition per load: unconditional ones took registers and a workgroup per CU with them (84 -> 116 us)
     if (a.n > 128 && count(256, 256) >= 256 && a.k % 64 == 0 && std::max(a.a.ld, a.b.ld) * (int64_t)sizeof(T) < (1 << 24))
       return la_go<T, MA, MB, 256, 256, 2, 4, EPI, true>(a, kLaGrid, st);
