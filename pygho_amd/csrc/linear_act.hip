@@ -98,6 +98,7 @@ static int64_t la_pad4(int64_t v) { return (v + 3) / 4 * 4; }
 //   stream  dz with the sums (and dX where W fits as that product needs it) from a streaming launch: 1.05 M rows of 256 -> 256 bf16 770 us,
 //           dX in a launch of its own 549 + 273
 //   else    dz by the row kernel from the pre-activation: kept by the forward, or (z) formed again in f32 where the forward streams
+// dz is in the rows' type everywhere: see linear_stream.h for what that rounding costs (its sums are taken before it)
 struct LaSpace { int64_t dz, z, sums, dw, wt, total; int nsum; bool fused, stream, own_dz; };
 static LaSpace la_space(int64_t m, int64_t k, int64_t n, int norm, int act, int dtype, bool aligned) {
   LaSpace s{};

@@ -508,7 +508,10 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC, size
         if constexpr (!DW) store_rows(reinterpret_cast<T*>(a.out), d, N);
         if constexpr (!DX && AHEAD) load_r(blk + stride);
         if constexpr (DX) {
-          // dz as the operand of dz . W: step s of n = this lane's registers 2 s, 2 s + 1 (16-bit, rounded once) or s (f32)
+          // dz as the operand of dz . W and dz^T x: step s of n = this lane's registers 2 s, 2 s + 1 (16-bit) or s (f32).  16-bit rows: dz is rounded to
+          // their type here, the one rounding of these operators that is not an output's -- the matrix cores take 16-bit operands, and a second
+          // term (dz - its rounding) would double the products of both gradients.  gx and gw are off by two independent roundings instead of one
+          // (bf16, relative to 64 bits: 0.0024 for 0.0017; the plain formula with dz rounded agrees to 0.0002); the sums above are of the f32 values
           uint4 f[G::NS];
 #pragma unroll
           for (int s = 0; s < G::NS; ++s) {

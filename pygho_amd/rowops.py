@@ -5,8 +5,10 @@ Row-wise MLP blocks without a batch norm (reference honn/utils.py:64-142: LayerN
     linear_act(x, W, b, act, residual)                      act(x W^T + b) + residual
     linear_norm_act(x, W, b, g, h, eps, act, residual)      act(LayerNorm(x W^T + b) * g + h) + residual
 
-over the last dim of x, any leading dims.  f32 / bf16 / f16; statistics and sums in f32, every output rounded once.  Parameters may be
-stored in x's dtype or (master weights) in f32; their gradients come back in their own dtype.  Gradients are first order only.
+over the last dim of x, any leading dims.  f32 / bf16 / f16; statistics and sums in f32, every output rounded once.  With 16-bit rows the gradient
+of x W^T + b enters the two products of the backward (x's and W's gradient) rounded to the rows' type, as the matrix cores take it; the gradients of
+bias and norm are sums of its f32 values.  Parameters may be stored in x's dtype or (master weights) in f32; their gradients come back in their own
+dtype.  Gradients are first order only.
 """
 from __future__ import annotations
 
