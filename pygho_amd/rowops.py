@@ -12,6 +12,7 @@ dtype.  Gradients are first order only.
 """
 from __future__ import annotations
 
+import math
 from typing import Optional, Tuple
 
 import torch
@@ -55,6 +56,18 @@ def _rows(t: Optional[Tensor], c: int) -> Tuple[Optional[Tensor], int]:
     if c > 1 and t2.stride(1) != 1:
         t2 = t2.contiguous()
     return t2, (t2.stride(0) if t2.shape[0] > 1 else c)
+
+
+def _device_rows(shape) -> Optional[Tensor]:
+    """the device-side count of the rows of a (.., C) tensor inside a batch slot (None: all rows are true ones).  As everywhere the extent of
+    dim 0 names the row family (`plans.row_families`); dims between it and the channels multiply its count"""
+    count = dyn_rows(shape[0]) if len(shape) > 1 else None
+    inner = math.prod(shape[1:-1])
+    if count is None or inner == 1:
+        return count
+    if shape[0] * inner > 2 ** 31 - 1:
+        raise RuntimeError(f"pygho_amd: {shape[0]} x {inner} rows of a batch slot pass the device-side row count's 32 bits")
+    return count[:1] * inner
 
 
 def _norm_params(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor]):
@@ -108,9 +121,9 @@ class _LayerNormAct(torch.autograd.Function):
         gw, gw_ptr, gw_code = _grad(need_w, c, w_dtype, dev)
         gb, gb_ptr, gb_code = _grad(need_b, c, b_dtype, dev)
         nbytes = int(lib().pygho_layer_norm_act_bwd_workspace(m, c))
-        ws = _workspace(nbytes, dev)
+        ws, count = _workspace(nbytes, dev), _device_rows(shape)
         check(lib().pygho_layer_norm_act_bwd(ptr(gx), gw_ptr, gw_code, gb_ptr, gb_code, ptr(x2), x_ld, ptr(gy2), gy_ld, ptr(w), ptr(b), pdt, m,
-                                             ptr(dyn_rows(m)), c, float(eps), ROW_ACT_CODE[act], code, ptr(ws), nbytes, stream_ptr(dev)),
+                                             ptr(count), c, float(eps), ROW_ACT_CODE[act], code, ptr(ws), nbytes, stream_ptr(dev)),
               "layer_norm_act_bwd")
         return (gx if need_x else None), gw, gb, (gy if need_r else None), None, None
 
@@ -192,9 +205,9 @@ class _LinearAct(torch.autograd.Function):
         gg, gg_ptr, gg_code = _grad(need_g, n, g_dtype, dev)
         gh, gh_ptr, gh_code = _grad(need_h, n, h_dtype, dev)
         nbytes = int(lib().pygho_linear_act_bwd_workspace(m, k, n, int(normed), ROW_ACT_CODE[act], code))
-        ws = _workspace(nbytes, dev)
+        ws, count = _workspace(nbytes, dev), _device_rows(x_shape)
         check(lib().pygho_linear_act_bwd(ptr(gx), gw_ptr, gw_code, gb_ptr, gb_code, gg_ptr, gg_code, gh_ptr, gh_code, ptr(z), ptr(x2), x_ld, ptr(w),
-                                         w_ld, ptr(b), bdt, int(normed), ptr(g), ptr(h), pdt, float(eps), ptr(gy2), gy_ld, m, ptr(dyn_rows(m)),
+                                         w_ld, ptr(b), bdt, int(normed), ptr(g), ptr(h), pdt, float(eps), ptr(gy2), gy_ld, m, ptr(count),
                                          k, n, ROW_ACT_CODE[act], code, ptr(ws), nbytes, stream_ptr(dev)), "linear_act_bwd")
         return gx, gw, gb, gg, gh, res, None, None, None
 
