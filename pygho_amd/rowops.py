@@ -167,7 +167,7 @@ class _LinearAct(torch.autograd.Function):
     (pygho_linear_act_keeps: W does not fit a CU's LDS), the pre-activation."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, g, h, residual, eps, act, normed):
+    def forward(ctx, x, weight, bias, g, h, residual, eps, act, normed, training):
         dt, dev = x.dtype, x.device
         n, k = weight.shape
         w, w_ld = _matrix(param_as(weight, dt).detach())
@@ -179,7 +179,8 @@ class _LinearAct(torch.autograd.Function):
         y = torch.empty(tuple(x.shape[:-1]) + (n,), dtype=dt, device=dev)
         keeps = int(lib().pygho_linear_act_keeps(k, n, int(normed), ROW_ACT_CODE[act], code))
         z = None
-        if keeps == 2 or (keeps == 1 and any(ctx.needs_input_grad[:5])):
+        # (`training`: the caller's grad mode.  In here it is always off, and needs_input_grad says what the inputs ask for in either mode)
+        if keeps == 2 or (keeps == 1 and training and any(ctx.needs_input_grad[:5])):
             z = torch.empty((m, n), dtype=torch.float32 if keeps == 2 else dt, device=dev)
         check(lib().pygho_linear_act(ptr(y), ptr(z), ptr(x2), x_ld, ptr(w), w_ld, ptr(b), bdt, int(normed), ptr(gg), ptr(hh), pdt, float(eps),
                                      ptr(r2), r_ld, m, k, n, ROW_ACT_CODE[act], code, stream_ptr(dev)), "linear_act")
@@ -193,7 +194,7 @@ class _LinearAct(torch.autograd.Function):
         need_x, need_w, need_b, need_g, need_h, need_r = ctx.needs_input_grad[:6]
         res = gy if need_r else None
         if not (need_x or need_w or need_b or need_g or need_h):
-            return None, None, None, None, None, res, None, None, None
+            return None, None, None, None, None, res, None, None, None, None
         x2, w, b, z, g, h = ctx.saved_tensors
         x_ld, w_ld, bdt, pdt, eps, act, normed, x_shape, w_dtype, b_dtype, g_dtype, h_dtype = ctx.meta
         n, k = w.shape
@@ -209,7 +210,7 @@ class _LinearAct(torch.autograd.Function):
         check(lib().pygho_linear_act_bwd(ptr(gx), gw_ptr, gw_code, gb_ptr, gb_code, gg_ptr, gg_code, gh_ptr, gh_code, ptr(z), ptr(x2), x_ld, ptr(w),
                                          w_ld, ptr(b), bdt, int(normed), ptr(g), ptr(h), pdt, float(eps), ptr(gy2), gy_ld, m, ptr(count),
                                          k, n, ROW_ACT_CODE[act], code, ptr(ws), nbytes, stream_ptr(dev)), "linear_act_bwd")
-        return gx, gw, gb, gg, gh, res, None, None, None
+        return gx, gw, gb, gg, gh, res, None, None, None, None
 
 
 def _linear_args(x: Tensor, weight: Tensor, bias: Optional[Tensor], act: str, residual: Optional[Tensor], what: str) -> None:
@@ -229,7 +230,7 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: st
     bias (N,): in x's dtype, or f32 master parameters (the product then takes W's copy in x's dtype, `param_as`), residual: the output's shape and
     x's dtype."""
     _linear_args(x, weight, bias, act, residual, "linear_act")
-    return _LinearAct.apply(x, weight, bias, None, None, residual, 0.0, act, False)
+    return _LinearAct.apply(x, weight, bias, None, None, residual, 0.0, act, False, torch.is_grad_enabled())
 
 
 def linear_norm_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, norm_weight: Optional[Tensor] = None,
@@ -245,4 +246,4 @@ def linear_norm_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, no
     if not eps >= 0:
         raise ValueError(f"pygho_amd.{what}: eps must not be negative")
     require_device(x, norm_weight, norm_bias)
-    return _LinearAct.apply(x, weight, bias, norm_weight, norm_bias, residual, eps, act, True)
+    return _LinearAct.apply(x, weight, bias, norm_weight, norm_bias, residual, eps, act, True, torch.is_grad_enabled())

@@ -99,3 +99,37 @@ def test_device_row_counts_under_more_dims_captured(dev):
         xe = x.detach()[:true].clone().requires_grad_(True)
         want = step(xe, gy[:true].clone())
         assert torch.equal(out[0][:true], want[0]) and torch.equal(out[1], want[1]), true
+
+
+# ---- prediction with parameters that could be trained --------------------------------------------------------------------------------
+def peak(f):
+    f()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    base = torch.cuda.memory_allocated()
+    out = f()
+    torch.cuda.synchronize()
+    return torch.cuda.max_memory_allocated() - base, out
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_prediction_keeps_no_pre_activation(dev, dtype):
+    """512 -> 512 with an activation is the form that keeps z for a gradient: without one only the output is allocated"""
+    from pygho_amd import _ops
+    x = torch.randn(20000, 512, device=dev).to(dtype)
+    w, b = torch.nn.Parameter(torch.randn(512, 512, device=dev).to(dtype)), torch.nn.Parameter(torch.randn(512, device=dev).to(dtype))
+    size = x.numel() * x.element_size()
+
+    def call():
+        return _ops.linear_act(x, w, b, "silu")
+    trained, y = peak(call)
+    assert trained >= 2 * size and y.requires_grad
+    with torch.no_grad():
+        spent, p = peak(call)
+    assert torch.equal(p, y.detach()) and not p.requires_grad and size <= spent < 1.1 * size
+    with torch.inference_mode():
+        spent, p = peak(call)
+    assert torch.equal(p, y.detach()) and size <= spent < 1.1 * size
+    # the residual alone needs a gradient: gy is all of it
+    spent, p = peak(lambda: _ops.linear_act(x, w.detach(), b.detach(), "silu", residual=x.detach().requires_grad_(True)))
+    assert p.requires_grad and spent < 1.1 * size
