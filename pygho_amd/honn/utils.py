@@ -207,7 +207,9 @@ class MLP(nn.Module):
 
     ``fused`` (an extension, same parameters and ``state_dict``): on device tensors every [Linear, LayerNorm | none, act] run is one operator
     (``_ops.linear_norm_act`` / ``_ops.linear_act``), the residual of ``forward`` included.  Under autocast such a block computes in the
-    autocast dtype from end to end (the stock modules return f32 from a LayerNorm); BatchNorm blocks are the same with and without it."""
+    autocast dtype from end to end (the stock modules return f32 from a LayerNorm); BatchNorm blocks are the same with and without it.  Modules
+    with hooks, a Linear whose class is not ``nn.Linear`` or this file's, other element types (f64) and weights that are neither in the compute
+    dtype nor f32 run as modules, as without the flag."""
 
     def __init__(self, hiddim: int, outdim: int, numlayer: int, tailact: bool, dp: float = 0, norm: str = "bn",
                  act: str = "relu", tailbias=True, normparam: float = 0.1, fused: bool = False) -> None:
@@ -312,16 +314,16 @@ class MLP(nn.Module):
         i = 0
         while i < len(mods):
             lin, i = mods[i], i + 1
-            if not isinstance(lin, nn.Linear):                 # an activation behind an active dropout, the dropout itself
+            if not _row_linear(lin, x):                        # an activation behind an active dropout, the dropout itself, modules of the user's own
                 x = lin(x)
                 continue
             norm = None
-            if i < len(mods) and type(mods[i]) in (LayerNorm, NoneNorm):
+            if i < len(mods) and type(mods[i]) in (LayerNorm, NoneNorm) and _unhooked(mods[i]):
                 norm = mods[i].norm if type(mods[i]) is LayerNorm else None
                 i += 1
-            if i < len(mods) and isinstance(mods[i], nn.Dropout) and not (mods[i].training and mods[i].p > 0):
+            if i < len(mods) and isinstance(mods[i], nn.Dropout) and _unhooked(mods[i]) and not (mods[i].training and mods[i].p > 0):
                 i += 1
-            act = _row_act(mods[i]) if i < len(mods) else None
+            act = _row_act(mods[i]) if i < len(mods) and _unhooked(mods[i]) else None
             if act is not None:
                 i += 1
             x = _autocast_input(x)
@@ -338,6 +340,23 @@ class MLP(nn.Module):
 
 
 _ACT_NAMES = {nn.SiLU: "silu", nn.ReLU: "relu"}
+
+
+_ROW_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _unhooked(mod: nn.Module) -> bool:
+    if mod._forward_hooks or mod._forward_pre_hooks or mod._backward_hooks or mod._backward_pre_hooks:
+        return False
+    return type(mod) is not LayerNorm or _unhooked(mod.norm)
+
+
+def _row_linear(mod: nn.Module, x: Tensor) -> bool:
+    """whether `mod` on `x` is a product that the row-wise operators form: a plain Linear without hooks, on a type that they take"""
+    if type(mod) not in (nn.Linear, Linear) or x.dtype not in _ROW_DTYPES or not _unhooked(mod):
+        return False
+    dt = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
+    return dt in _ROW_DTYPES and mod.weight.dtype in (dt, torch.float32)
 
 
 def _row_act(mod: nn.Module) -> Optional[str]:

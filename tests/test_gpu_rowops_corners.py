@@ -133,3 +133,57 @@ def test_prediction_keeps_no_pre_activation(dev, dtype):
     # the residual alone needs a gradient: gy is all of it
     spent, p = peak(lambda: _ops.linear_act(x, w.detach(), b.detach(), "silu", residual=x.detach().requires_grad_(True)))
     assert p.requires_grad and spent < 1.1 * size
+
+
+# ---- what the fused MLP leaves to the stock modules ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("norm", ["ln", "none"])
+def test_fused_mlp_leaves_other_types_to_the_stock_modules(dev, norm):
+    from pygho_amd.honn.utils import MLP
+    torch.manual_seed(0)
+    stock, fused = (MLP(40, 24, 2, True, norm=norm, act="silu", fused=f).to(dev).double() for f in (False, True))
+    fused.load_state_dict(stock.state_dict())
+    x, r = torch.randn(33, 40, device=dev, dtype=torch.float64), torch.randn(33, 24, device=dev, dtype=torch.float64)
+    out = []
+    for m in (stock, fused):
+        xx = x.clone().requires_grad_(True)
+        y = m(xx, residual=r)
+        out.append((y.detach(), *torch.autograd.grad(y.sum(), [xx, *m.parameters()])))
+    assert out[1][0].dtype == torch.float64 and all(torch.equal(a, b) for a, b in zip(*out))
+
+
+def test_fused_mlp_runs_hooks_and_modules_of_the_users_own(dev):
+    """a hook on an inner module, a Linear whose forward is another, a weight under a parametrization: their code runs"""
+    from pygho_amd.honn.utils import MLP
+    torch.manual_seed(0)
+    x = torch.randn(33, 40, device=dev)
+
+    def model():
+        torch.manual_seed(1)
+        return MLP(40, 40, 2, True, norm="ln", act="silu", fused=True).to(dev)
+    plain, seen = model()(x), []
+    for i in range(6):
+        m = model()
+        seen.clear()
+        handle = m.lins[i].register_forward_hook(lambda mod, args, out: seen.append(type(mod).__name__))
+        try:
+            assert float((m(x) - plain).abs().max()) < 1e-5 and seen       # (activations are shared between the blocks: once or twice)
+        finally:
+            handle.remove()
+        assert torch.equal(m(x), plain)
+    m = model()
+    m.lins[1].norm.register_forward_pre_hook(lambda mod, args: seen.append("norm"))
+    m(x)
+    assert seen[-1] == "norm"
+
+    class Doubled(torch.nn.Linear):
+        def forward(self, t):
+            return 2.0 * super().forward(t)
+    m = model()
+    own = Doubled(40, 40).to(dev)
+    own.load_state_dict(m.lins[0].state_dict())
+    m.lins[0] = own
+    want = m.lins[5](m.lins[4](m.lins[3](m.lins[2](m.lins[1](own(x))))))
+    assert float((m(x) - want).abs().max()) < 1e-5
+    m = model()
+    torch.nn.utils.parametrizations.weight_norm(m.lins[3])
+    assert float((m(x) - plain).abs().max()) < 1e-5
