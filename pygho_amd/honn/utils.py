@@ -326,9 +326,9 @@ class MLP(nn.Module):
             act = _row_act(mods[i]) if i < len(mods) and _unhooked(mods[i]) else None
             if act is not None:
                 i += 1
-            x = _autocast_input(x)
-            res = residual if (residual is not None and i == len(mods) and residual.dtype == x.dtype
-                               and residual.shape == tuple(x.shape[:-1]) + (lin.out_features,)) else None
+            x = _near_rows(_autocast_input(x))
+            res = _near_rows(residual) if (residual is not None and i == len(mods) and residual.dtype == x.dtype
+                                           and residual.shape == tuple(x.shape[:-1]) + (lin.out_features,)) else None
             with torch.autocast("cuda", enabled=False):
                 if norm is None:
                     x = _ops.linear_act(x, lin.weight, lin.bias, act or "none", residual=res)
@@ -357,6 +357,12 @@ def _row_linear(mod: nn.Module, x: Tensor) -> bool:
         return False
     dt = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
     return dt in _ROW_DTYPES and mod.weight.dtype in (dt, torch.float32)
+
+
+def _near_rows(t: Tensor) -> Tensor:
+    """`t`, copied where its rows are 2^27 bytes or more apart (the linear operators reach a block of rows with 32-bit offsets)"""
+    far = not t.is_contiguous() and any(d > 1 and s * t.element_size() >= 1 << 27 for d, s in zip(t.shape[:-1], t.stride()))
+    return t.contiguous() if far else t
 
 
 def _row_act(mod: nn.Module) -> Optional[str]:

@@ -48,12 +48,13 @@ def _row_operand(t: Optional[Tensor], shape, dtypes, name: str, what: str) -> No
         raise TypeError(f"pygho_amd.{what}: {name} is {t.dtype}, needs {' or '.join(str(d) for d in dtypes)}")
 
 
-def _rows(t: Optional[Tensor], c: int) -> Tuple[Optional[Tensor], int]:
-    """(rows, width) view of t and its row stride in elements; a copy only where the channels of a row are not adjacent"""
+def _rows(t: Optional[Tensor], c: int, within: int = 0) -> Tuple[Optional[Tensor], int]:
+    """(rows, width) view of t and its row stride in elements; a copy where the channels of a row are not adjacent, where the leading dims do
+    not merge into one stride, and where the rows are `within` bytes or more apart (0: any distance)"""
     if t is None:
         return None, 0
     t2 = t if t.dim() == 2 else t.reshape(-1, c)
-    if c > 1 and t2.stride(1) != 1:
+    if (c > 1 and t2.stride(1) != 1) or (within and t2.shape[0] > 1 and t2.stride(0) * t2.element_size() >= within):
         t2 = t2.contiguous()
     return t2, (t2.stride(0) if t2.shape[0] > 1 else c)
 
@@ -198,7 +199,7 @@ class _LinearAct(torch.autograd.Function):
         x2, w, b, z, g, h = ctx.saved_tensors
         x_ld, w_ld, bdt, pdt, eps, act, normed, x_shape, w_dtype, b_dtype, g_dtype, h_dtype = ctx.meta
         n, k = w.shape
-        gy2, gy_ld = _rows(gy, n)
+        gy2, gy_ld = _rows(gy, n, 1 << 27)                     # (the caller of a forward chose its strides, nobody chooses a gradient's)
         m, dev, code = x2.shape[0], x2.device, DTYPE_CODE[x2.dtype]
         gx = torch.empty(x_shape, dtype=x2.dtype, device=dev) if need_x else None
         gw, gw_ptr, gw_code = _grad(need_w, (n, k), w_dtype, dev)
@@ -228,7 +229,7 @@ def _linear_args(x: Tensor, weight: Tensor, bias: Optional[Tensor], act: str, re
 def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: str = "none", residual: Optional[Tensor] = None) -> Tensor:
     """act(x @ weight^T + bias) + residual over the last dim of x in one launch; act is one of "none", "relu", "silu", "elu".  weight (N, K) and
     bias (N,): in x's dtype, or f32 master parameters (the product then takes W's copy in x's dtype, `param_as`), residual: the output's shape and
-    x's dtype."""
+    x's dtype.  Rows of x and residual less than 2^27 bytes apart."""
     _linear_args(x, weight, bias, act, residual, "linear_act")
     return _LinearAct.apply(x, weight, bias, None, None, residual, 0.0, act, False, torch.is_grad_enabled())
 

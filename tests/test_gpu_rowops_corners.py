@@ -187,3 +187,22 @@ def test_fused_mlp_runs_hooks_and_modules_of_the_users_own(dev):
     m = model()
     torch.nn.utils.parametrizations.weight_norm(m.lins[3])
     assert float((m(x) - plain).abs().max()) < 1e-5
+
+
+def test_fused_mlp_on_rows_far_apart(dev):
+    """rows 2^27 bytes apart, which the operators refuse: the MLP takes a copy.  A gradient that arrives that way as well"""
+    from pygho_amd import _ops
+    from pygho_amd.honn.utils import MLP
+    torch.manual_seed(0)
+    m = MLP(128, 128, 1, True, norm="ln", act="silu", fused=True).to(dev)
+    x, gy = torch.randn(2, 128, device=dev), torch.randn(2, 128, device=dev)
+    room = torch.empty((1 << 25) + 1024, device=dev)
+    far, gfar = room.as_strided((2, 128), (1 << 25, 1)), room.as_strided((2, 128), (1 << 25, 1), 512)
+    far.copy_(x)
+    gfar.copy_(gy)
+    with pytest.raises(RuntimeError, match="strides"):
+        _ops.linear_act(far, m.lins[0].weight)
+    assert torch.equal(m(far, residual=far), m(x, residual=x))
+    t = x.clone().requires_grad_(True)
+    got, want = (torch.autograd.grad(m(t), [t, *m.parameters()], g) for g in (gfar, gy))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
