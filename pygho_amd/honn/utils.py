@@ -211,6 +211,8 @@ class MLP(nn.Module):
     with hooks, a Linear whose class is not ``nn.Linear`` or this file's, other element types (f64) and weights that are neither in the compute
     dtype nor f32 run as modules, as without the flag."""
 
+    fused = False                                              # (a whole module that was pickled before the flag existed has no such attribute)
+
     def __init__(self, hiddim: int, outdim: int, numlayer: int, tailact: bool, dp: float = 0, norm: str = "bn",
                  act: str = "relu", tailbias=True, normparam: float = 0.1, fused: bool = False) -> None:
         super().__init__()

@@ -14,3 +14,14 @@ def test_device_row_counts_past_32_bits_are_refused():
             rowops._device_rows((50000, 50000, 64))
     finally:
         del plans._ROW_FAMILIES[50000]
+
+
+def test_an_mlp_pickled_before_the_flag_still_runs():
+    import copy
+    from pygho_amd.honn.utils import MLP
+    torch.manual_seed(0)
+    a = MLP(8, 8, 2, True, norm="ln", act="silu")
+    b = copy.deepcopy(a)
+    b.__dict__.pop("fused", None)                              # what unpickling an instance of the earlier class gives
+    x = torch.randn(5, 8)
+    assert torch.equal(a(x, residual=x), b(x, residual=x))
