@@ -48,7 +48,12 @@ def _capture_mode() -> str:
     mode ("global") refuses -- the watchdog then ends the process ("operation not permitted when stream is capturing").  Queries of another
     thread touch nothing that is being captured, so with such a group only the capturing thread is held to the rules."""
     import torch.distributed as dist
-    return "thread_local" if dist.is_available() and dist.is_initialized() and "nccl" in str(dist.get_backend()) else "global"
+    if not (dist.is_available() and dist.is_initialized()):
+        return "global"
+    # every group of this process, by its backend per device: the default group's name is "undefined" when none was asked for, and a group made
+    # with new_group may have RCCL where the default one has not
+    backends = [dist.get_backend()] + [dist.get_backend_config(group) for group in list(dist.distributed_c10d._world.pg_map)]
+    return "thread_local" if any("nccl" in str(b) for b in backends) else "global"
 
 
 class GraphedStep:
