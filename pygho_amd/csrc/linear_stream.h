@@ -550,7 +550,9 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC, size
           char* base = reinterpret_cast<char*>(a.gx) + blk * 16 * K * ES;
           const uint32_t row = (uint32_t)r16 * (uint32_t)(K * ES);
           const int kb_end = DW && !a.gx ? 0 : (K + 15) / 16;
-          constexpr int KG = NORM ? 2 : 4;                     // 16-channel blocks at once (the norm's registers leave room for two)
+          // 16-channel blocks at once: two where the norm's or 128 f32 channels' registers leave room for no more (f32 262144 x 96 -> 112 gradients
+          // 261 us, with four 279; 1.05 M x 128 -> 128 1050, 1055)
+          constexpr int KG = NORM || (ES == 4 && NB == 8) ? 2 : 4;
           for (int kg = 0; kg < kb_end; kg += KG) {
             la_f32x4_t o[KG];
 #pragma unroll

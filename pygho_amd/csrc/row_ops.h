@@ -11,10 +11,11 @@ namespace pygho {
 // enum pygho_row_act (pygho_hip.h)
 constexpr int kActNone = PYGHO_ACT_NONE, kActRelu = PYGHO_ACT_RELU, kActSilu = PYGHO_ACT_SILU, kActElu = PYGHO_ACT_ELU;
 
-// f32 storage takes the library's correctly rounded-ish exp / expm1 / divide (their error must stay below 2^-24 of the result); 16-bit
-// storage the hardware exp2 and reciprocal (1 ulp of f32 each, 2^-13 of a 16-bit half step)
+// f32 storage takes the library's expf and expm1f (about one ulp) and the correctly rounded divide; 16-bit storage the hardware exp2 and
+// reciprocal (1 ulp of f32 each, 2^-13 of a 16-bit half step)
 template <typename T> struct Precise { static constexpr bool value = std::is_same<T, float>::value; };
 
+template <bool P> __device__ __forceinline__ float ro_exp(float z) { return P ? expf(z) : __expf(z); }
 template <bool P> __device__ __forceinline__ float ro_sigmoid(float z) {
   if constexpr (P) return 1.f / (1.f + expf(-z));
   return __builtin_amdgcn_rcpf(1.f + __expf(-z));
@@ -54,7 +55,7 @@ template <bool P, int N> __device__ __forceinline__ void ro_act_slope(float (&g)
     for (int i = 0; i < N; ++i) g[i] = z[i] <= 0.f ? 0.f : g[i];
   } else if (act == kActElu) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) g[i] *= z[i] <= 0.f ? ro_expm1<P>(z[i]) + 1.f : 1.f;
+    for (int i = 0; i < N; ++i) g[i] *= z[i] <= 0.f ? ro_exp<P>(z[i]) : 1.f;          // (not expm1 + 1: that is 0 below -17)
   }
 }
 

@@ -30,6 +30,48 @@ def same(got, want, tol, what):
         raise AssertionError(f"{what}: {int((~ok).sum())} of {ok.numel()} off, first at {i}: got {got.flatten()[i].item()!r}, want {want.flatten()[i].item()!r}")
 
 
+# ---- the slope of elu far below zero ------------------------------------------------------------------------------------------------
+# exp(u) in f32 for u exact: the rounding of u log2(e) moves the exponential by |u| 2^-24 relative, exp2 / expf and the product by 2^-22 at most;
+# the sums are of terms of one sign, at most 400 of them in any order: (|u| + 4 + 400) 2^-24 covers all of it
+DEEP = 512 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [16, 64, 100, 128, 256, 300, 512])
+def test_elu_slope_far_below_zero_linear(dev, dtype, n):
+    """W = identity: z is x and gx the gradient of z itself.  expm1(z) + 1 would be 0 below -17 and 1e-3 off at -12"""
+    from pygho_amd import _ops
+    m = 90
+    x = -8.0 - 0.25 * (torch.arange(m * n, device=dev) % 89).reshape(m, n)                        # -8 .. -30, exact in every type
+    x, w, b = x.to(dtype), torch.eye(n, device=dev, dtype=dtype), torch.zeros(n, device=dev)
+    gy = (1.0 + (torch.arange(m * n, device=dev) % 4).reshape(m, n)).to(dtype)
+    t = [x.requires_grad_(True), w.requires_grad_(True), b.requires_grad_(True)]
+    gx, gw, gb = torch.autograd.grad(_ops.linear_act(*t, act="elu"), t, gy)
+    dz = gy.double() * torch.exp(x.detach().double())
+    same(gx, dz, dz * (2 * HALF[dtype] + DEEP) + 2 * TINY[dtype], f"gx {n}")                         # (16-bit: dz is rounded, then the result)
+    same(gb, dz.sum(0), dz.sum(0) * (HALF[torch.float32] + DEEP), f"gb {n}")
+    want, size = dz.t() @ x.detach().double(), dz.t() @ x.detach().double().abs()
+    same(gw, want, size * (2 * HALF[dtype] + DEEP) + m * 40 * TINY[dtype], f"gw {n}")                # dz of f16 may be subnormal: m rows of |x| <= 30
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("c", [16, 100, 128, 257, 1000, 2056])
+def test_elu_slope_far_below_zero_norm(dev, dtype, c):
+    """a norm whose weight is zero hands its bias to the activation: gbias = sum gy exp(bias)"""
+    from pygho_amd import _ops
+    m = 90
+    h = (-8.0 - 0.25 * (torch.arange(c, device=dev) % 89)).requires_grad_(True)
+    g = torch.zeros(c, device=dev, requires_grad=True)
+    x = torch.randn(m, c, generator=torch.Generator(device=dev).manual_seed(c), device=dev).to(dtype)
+    gy = (1.0 + (torch.arange(m * c, device=dev) % 4).reshape(m, c)).to(dtype)
+    want = (gy.double() * torch.exp(h.detach().double())).sum(0)
+    gh, = torch.autograd.grad(_ops.layer_norm_act(x, g, h, act="elu"), h, gy)
+    same(gh, want, want * (HALF[torch.float32] + DEEP), f"layer_norm_act {c}")
+    w = torch.randn(c, 32, generator=torch.Generator(device=dev).manual_seed(c), device=dev).to(dtype)
+    gh, = torch.autograd.grad(_ops.linear_norm_act(x[:, :16].repeat(1, 2), w, None, g, h, act="elu"), h, gy)
+    same(gh, want, want * (HALF[torch.float32] + DEEP), f"linear_norm_act {c}")
+
+
 # ---- rows counted on the device: the family is named by the extent of dim 0 ------------------------------------------------------------
 def calls(_ops, k, n, gen, dev, dtype):
     p = [torch.randn(s, generator=gen, device=dev).div_(4).to(dtype).requires_grad_(True) for s in ((n, k), (n,), (n,), (n,), (k,), (k,))]
