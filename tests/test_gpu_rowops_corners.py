@@ -72,6 +72,36 @@ def test_elu_slope_far_below_zero_norm(dev, dtype, c):
     same(gh, want, want * (HALF[torch.float32] + DEEP), f"linear_norm_act {c}")
 
 
+# ---- a pre-activation that is kept in 16 bits ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("act", ["silu", "elu", "relu"])
+@pytest.mark.parametrize("k,n", [(128, 128), (256, 256), (300, 300), (512, 512)])
+def test_f16_pre_activations_beyond_the_type(dev, k, n, act):
+    """|z| of 2 or 4 times f16's largest value: the slope is 0 or 1, in the forms that keep z as in those that form it again; dz is gy or 0 and every
+    sum below exact.  An infinity that the input holds stays one"""
+    from pygho_amd import _ops
+    m = 40
+    sign = torch.where(torch.arange(n, device=dev) % 2 == 0, 1.0, -1.0)
+    x = torch.full((m, k), 1024.0, device=dev, dtype=torch.float16)
+    w = (sign[:, None] * (1.0 if k <= 256 else 0.5)).expand(n, k).contiguous().half()
+    gy = (torch.arange(m * n, device=dev) % 3 - 1).reshape(m, n).half()
+    x.requires_grad_(True), w.requires_grad_(True)
+    y = _ops.linear_act(x, w, None, act)
+    gx, gw = torch.autograd.grad(y, (x, w), gy)
+    z = x.detach().double() @ w.detach().double().t()
+    assert float(z.abs().min()) > 65504 * 1.9
+    dz = gy.double() * (z > 0)
+    low = {"silu": 0.0, "elu": -1.0, "relu": 0.0}[act]
+    assert torch.equal(y.detach(), torch.where(z > 0, z, torch.full_like(z, low)).half())
+    assert torch.equal(gx, (dz @ w.detach().double()).half())
+    assert torch.equal(gw, (dz.t() @ x.detach().double()).half())
+    if act == "silu":
+        bad = x.detach().clone()
+        bad[3, 5] = float("inf")
+        bad.requires_grad_(True)
+        gx, = torch.autograd.grad(_ops.linear_act(bad, w.detach(), None, act), bad, torch.ones_like(gy))
+        assert bool(torch.isnan(gx[3]).all()) and bool(torch.isfinite(gx[:3]).all()) and bool(torch.isfinite(gx[4:]).all())
+
+
 # ---- rows counted on the device: the family is named by the extent of dim 0 ------------------------------------------------------------
 def calls(_ops, k, n, gen, dev, dtype):
     p = [torch.randn(s, generator=gen, device=dev).div_(4).to(dtype).requires_grad_(True) for s in ((n, k), (n,), (n,), (n,), (k,), (k,))]
