@@ -317,7 +317,12 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC, size
     if constexpr (AHEAD) load_r(blk);
   }
   for (; (DW ? blk - wave : blk) < n_blocks; blk += stride) {
+    const bool row_ok = r16 <= (int)min((int64_t)15, m_rows - 1 - blk * 16);
     if constexpr (DW) {
+      if ((blk + 1) * 16 > m_rows) {                           // a repeated row's dz is zero; its x has to be as well: 0 * inf would be NaN
+#pragma unroll
+        for (int s = 0; s < KC; ++s) xc[s] = row_ok ? xc[s] : make_uint4(0u, 0u, 0u, 0u);
+      }
       __syncthreads();                                         // the stage is read
 #pragma unroll
       for (int s = 0; s < KC; ++s)
@@ -327,7 +332,6 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC, size
     asm volatile("" ::: "memory");
     int N_here = N;
     asm volatile("" : "+s"(N_here));
-    const bool row_ok = r16 <= (int)min((int64_t)15, m_rows - 1 - blk * 16);
     if constexpr (!AHEAD) load_r(blk);
     if (BWD && (blk + 1) * 16 > m_rows) {                      // a repeated row adds nothing to the sums: its gradient is zero
 #pragma unroll

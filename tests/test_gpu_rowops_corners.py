@@ -102,6 +102,28 @@ def test_f16_pre_activations_beyond_the_type(dev, k, n, act):
         assert bool(torch.isnan(gx[3]).all()) and bool(torch.isfinite(gx[:3]).all()) and bool(torch.isfinite(gx[4:]).all())
 
 
+# ---- infinities in the last row ----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k,n", [(128, 128), (64, 64), (96, 112), (100, 36), (384, 128), (256, 256), (512, 512)])
+@pytest.mark.parametrize("m", [1, 17, 333, 2000])
+def test_an_infinity_in_the_last_row_counts_once(dev, dtype, m, k, n):
+    """the weight's gradient is infinite where that row's dz is not zero, NaN where it is (0 * inf), and finite in the other columns -- whatever a
+    launch does with the lanes behind the last row.  Small integers: everything finite is exact"""
+    from pygho_amd import _ops
+    gen = torch.Generator(device=dev).manual_seed(m + k + n)
+    x = torch.randint(-2, 3, (m, k), generator=gen, device=dev).to(dtype)
+    w = (torch.randint(0, 2, (n, k), generator=gen, device=dev) * 2 - 1).to(dtype)              # no zeros: z of that row is +-inf, never NaN
+    gy = torch.randint(1, 3, (m, n), generator=gen, device=dev).to(dtype)
+    x[m - 1, 7] = float("inf")
+    z = x.double() @ w.double().t()
+    dz = gy.double() * (z > 0)
+    t = [x.requires_grad_(True), w.requires_grad_(True)]
+    gw, = torch.autograd.grad(_ops.linear_act(*t, act="relu"), t[1:], gy)
+    want = dz.t() @ x.detach().double()
+    assert bool(torch.isinf(want[:, 7]).any()) and bool(torch.isnan(want[:, 7]).any()) and bool(torch.isfinite(want[:, :7]).all())
+    same(gw, want.to(dtype).double(), torch.zeros_like(want), f"{m} x {k} -> {n}")
+
+
 # ---- rows counted on the device: the family is named by the extent of dim 0 ------------------------------------------------------------
 def calls(_ops, k, n, gen, dev, dtype):
     p = [torch.randn(s, generator=gen, device=dev).div_(4).to(dtype).requires_grad_(True) for s in ((n, k), (n,), (n,), (n,), (k,), (k,))]
