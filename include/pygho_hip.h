@@ -882,7 +882,11 @@ int pygho_linear_act_keeps(int64_t k, int64_t n, int norm, int act, int dtype);
 int pygho_linear_act(void* y, void* z, const void* x, int64_t x_ld, const void* w, int64_t w_ld, const void* bias, int bias_dtype, int norm,
                      const void* g, const void* h, int norm_dtype, double eps, const void* residual, int64_t residual_ld, int64_t m, int64_t k,
                      int64_t n, int act, int dtype, void* stream);
+/* bytes of workspace: for any gradients and operands of that size, and (_for) for a call with just these -- gx and the operands are looked at for
+ * NULL and alignment only.  Without gw and gb no weight-gradient space, without gw no more than the sums where dz need not reach memory */
 size_t pygho_linear_act_bwd_workspace(int64_t m, int64_t k, int64_t n, int norm, int act, int dtype);
+size_t pygho_linear_act_bwd_workspace_for(const void* gx, int want_gw, int want_gb, const void* x, int64_t x_ld, const void* gy, int64_t gy_ld,
+                                          int64_t m, int64_t k, int64_t n, int norm, int act, int dtype);
 int pygho_linear_act_bwd(void* gx, void* gw, int gw_dtype, void* gb, int gb_dtype, void* gg, int gg_dtype, void* gh, int gh_dtype, const void* z,
                          const void* x, int64_t x_ld, const void* w, int64_t w_ld, const void* bias, int bias_dtype, int norm, const void* g,
                          const void* h, int norm_dtype, double eps, const void* gy, int64_t gy_ld, int64_t m_cap, const int32_t* m_dev, int64_t k,

@@ -158,6 +158,7 @@ PROTOTYPES = {
     "pygho_linear_act_keeps": (I, [L, L, I, I, I]),
     "pygho_linear_act": (I, [P, P, P, L, P, L, P, I, I, P, P, I, D, P, L, L, L, L, I, I, P]),
     "pygho_linear_act_bwd_workspace": (Z, [L, L, L, I, I, I]),
+    "pygho_linear_act_bwd_workspace_for": (Z, [P, I, I, P, L, P, L, L, L, L, I, I, I]),
     "pygho_linear_act_bwd": (I, [P, P, I, P, I, P, I, P, I, P, P, L, P, L, P, I, I, P, P, I, D, P, L, L, P, L, L, I, I, P, Z, P]),
 }
 

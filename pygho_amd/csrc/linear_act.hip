@@ -56,16 +56,20 @@ static int la_form(int64_t k, int64_t n, int norm, int dtype) {
 static int la_forward(const LsArgs& a, int form, int norm, int dtype, hipStream_t st) {
   return la_type(dtype, [&](auto ops) { return form == FORM_OUT ? ops.out_fwd(a, st) : ops.stream_fwd(a, norm, st); });
 }
+// whether x, the rows of gy and what is stored beside them allow the unmasked accesses of linear_stream.h
+static int la_vec(const void* x, int64_t x_ld, const void* r, int64_t r_ld, const void* out, int64_t k, int64_t n, int dtype) {
+  const int es = la_size(dtype);
+  return (k % (64 / es) == 0 && la_aligned(x, x_ld, es, 16) ? 1 : 0) | (n % 16 == 0 && la_aligned(r, r_ld, es, 16) && la_aligned(out, n, es, 16) ? 2 : 0);
+}
 static LsArgs la_stream_args(const void* x, int64_t x_ld, const void* w, int64_t w_ld, const void* bias, int bias_dtype, const void* g, const void* h,
                              int norm_dtype, const void* r, int64_t r_ld, void* out, int64_t m, int64_t k, int64_t n, double eps, int act, int dtype) {
-  const int es = la_size(dtype);
   LsArgs a{};
   a.x = x; a.x_ld = x_ld;
   a.w = w; a.w_ld = w_ld;
   a.bias = bias; a.bias_dtype = bias_dtype; a.g = g; a.h = h; a.norm_dtype = norm_dtype;
   a.r = r; a.r_ld = r_ld;
   a.out = out;
-  a.vec = (k % (64 / es) == 0 && la_aligned(x, x_ld, es, 16) ? 1 : 0) | (n % 16 == 0 && la_aligned(r, r_ld, es, 16) && la_aligned(out, n, es, 16) ? 2 : 0);
+  a.vec = la_vec(x, x_ld, r, r_ld, out, k, n, dtype);
   a.m = m; a.k = (int)k; a.n = (int)n; a.eps = (float)eps; a.act = act;
   return a;
 }
@@ -93,31 +97,40 @@ static int64_t la_dw_slabs(int64_t m, int64_t k, int64_t n) {
 static int64_t la_pad4(int64_t v) { return (v + 3) / 4 * 4; }
 
 // The launches of a backward pass and its workspace, in bytes: [dz] [z] [slabs of the sums over n] [slabs of dW | db] [W^T]
-//   fused   dz, dX, dW and every sum from one streaming launch (operands aligned; its slabs are [sums | dW]): 1.05 M rows of 128 -> 64 / 128 bf16
-//           151 / 220 us, in separate launches 261 / 357
+//   fused   dz, dX, dW and every sum from one streaming launch (dW asked for, operands aligned; its slabs are [sums | dW]): 1.05 M rows of 128 -> 64 / 128
+//           bf16 151 / 220 us, in separate launches 261 / 357
 //   stream  dz with the sums (and dX where W fits as that product needs it) from a streaming launch: 1.05 M rows of 256 -> 256 bf16 770 us,
 //           dX in a launch of its own 549 + 273
 //   else    dz by the row kernel from the pre-activation: kept by the forward, or (z) formed again in f32 where the forward streams
-// dz is in the rows' type everywhere: see linear_stream.h for what that rounding costs (its sums are taken before it)
-struct LaSpace { int64_t dz, z, sums, dw, wt, total; int nsum; bool fused, stream, own_dz; };
-static LaSpace la_space(int64_t m, int64_t k, int64_t n, int norm, int act, int dtype, bool aligned) {
+// dz is in the rows' type everywhere: see linear_stream.h for what that rounding costs (its sums are taken before it).  It reaches memory where a later
+// launch reads it
+struct LaAsk { bool gx, gw, gb, aligned; };                    // the gradients of a call; aligned: VEC 3 of linear_stream.h
+struct LaSpace { int64_t dz, z, sums, dw, wt, total; int nsum; int64_t dw_k; bool fused, stream, own_dz, gx_here; };
+static LaSpace la_space(int64_t m, int64_t k, int64_t n, int norm, int act, int dtype, const LaAsk& ask) {
   LaSpace s{};
   s.nsum = norm ? 3 : 1;
-  const int64_t slabs = std::min<int64_t>(kLsGrid, ceil_div(m, 16));      // a streaming launch: at most one workgroup per block of rows
-  s.fused = aligned && la_type(dtype, [&](auto ops) { return ops.dw_fits(k, n, s.nsum); });
+  s.fused = ask.gw && ask.aligned && la_type(dtype, [&](auto ops) { return ops.dw_fits(k, n, s.nsum); });
   if (s.fused) {
-    s.total = s.dw = slabs * la_pad4(s.nsum * n + n * k) * 4;
+    s.total = s.dw = std::min<int64_t>(kLsDwGrid, ceil_div(m, 16 * kLsDwWaves)) * la_pad4(s.nsum * n + n * k) * 4;
     return s;
   }
   s.own_dz = norm || act != kActNone;
   s.stream = s.own_dz && n <= ls_bwd_max(norm, la_size(dtype)) && la_type(dtype, [&](auto ops) { return ops.stream_lds(k, n, s.nsum, false, false) <= kLsLds; });
-  s.dz = s.own_dz ? (m * n * la_size(dtype) + 15) / 16 * 16 : 0;
+  s.gx_here = ask.gx && s.stream && la_type(dtype, [&](auto ops) { return ops.stream_lds(k, n, s.nsum, true, false) <= kLsLds; });
+  const bool gx_later = ask.gx && !s.gx_here, db = ask.gb && !s.own_dz;     // (dz = gy: its column sums come with dW, or with 16 columns of it)
+  s.dw_k = ask.gw ? k : db ? std::min<int64_t>(k, 16) : 0;
+  s.dz = s.own_dz && (!s.stream || ask.gw || gx_later) ? (m * n * la_size(dtype) + 15) / 16 * 16 : 0;
   s.z = s.own_dz && !s.stream && la_form(k, n, norm, dtype) != FORM_TILE ? (m * n * 4 + 15) / 16 * 16 : 0;
+  const int64_t slabs = std::min<int64_t>(kLsGrid, ceil_div(m, 16));      // a streaming launch: at most one workgroup per block of rows
   s.sums = !s.own_dz ? 0 : s.stream ? slabs * la_pad4(s.nsum * n) * 4 : ln_bwd_slab_floats(m, n, s.nsum) * 4;
-  s.dw = la_dw_slabs(m, k, n) * la_pad4(n * k + n) * 4;
-  s.wt = la_form(n, k, 0, dtype) == FORM_TILE ? (n * k * la_size(dtype) + 15) / 16 * 16 : 0;
+  s.dw = s.dw_k ? la_dw_slabs(m, s.dw_k, n) * la_pad4(n * s.dw_k + n) * 4 : 0;
+  s.wt = gx_later && la_form(n, k, 0, dtype) == FORM_TILE ? (n * k * la_size(dtype) + 15) / 16 * 16 : 0;
   s.total = s.dz + s.z + s.sums + s.dw + s.wt;
   return s;
+}
+static int la_vec_bwd(const void* gx, const void* x, int64_t x_ld, const void* gy, int64_t gy_ld, int64_t k, int64_t n, int dtype) {
+  const int vec = la_vec(x, x_ld, gy, gy_ld, nullptr, k, n, dtype);       // (dz's place in the workspace is aligned; dX is stored in the same launch)
+  return gx && !(k % 16 == 0 && la_aligned(gx, k, la_size(dtype), 16)) ? vec & 1 : vec;
 }
 
 }  // namespace pygho
@@ -151,7 +164,13 @@ extern "C" int pygho_linear_act(void* y, void* z, const void* x, int64_t x_ld, c
 
 extern "C" size_t pygho_linear_act_bwd_workspace(int64_t m, int64_t k, int64_t n, int norm, int act, int dtype) {
   if (m <= 0 || k <= 0 || n <= 0 || !ro_float(dtype)) return 0;
-  return (size_t)std::max(la_space(m, k, n, norm, act, dtype, true).total, la_space(m, k, n, norm, act, dtype, false).total);
+  return (size_t)std::max(la_space(m, k, n, norm, act, dtype, LaAsk{true, true, true, true}).total, la_space(m, k, n, norm, act, dtype, LaAsk{true, true, true, false}).total);
+}
+
+extern "C" size_t pygho_linear_act_bwd_workspace_for(const void* gx, int want_gw, int want_gb, const void* x, int64_t x_ld, const void* gy, int64_t gy_ld,
+                                                     int64_t m, int64_t k, int64_t n, int norm, int act, int dtype) {
+  if (m <= 0 || k <= 0 || n <= 0 || !ro_float(dtype)) return 0;
+  return (size_t)la_space(m, k, n, norm, act, dtype, LaAsk{gx != nullptr, want_gw != 0, want_gb != 0, la_vec_bwd(gx, x, x_ld, gy, gy_ld, k, n, dtype) == 3}).total;
 }
 
 extern "C" int pygho_linear_act_bwd(void* gx, void* gw, int gw_dtype, void* gb, int gb_dtype, void* gg, int gg_dtype, void* gh, int gh_dtype,
@@ -172,16 +191,16 @@ extern "C" int pygho_linear_act_bwd(void* gx, void* gw, int gw_dtype, void* gb, 
     if (int rc = fold_launch(FoldOut{{gw, gb, gg, gh}, {gw ? n * k : 0, gb ? n : 0, gg ? n : 0, gh ? n : 0}, {gw_dtype, gb_dtype, gg_dtype, gh_dtype}}, nullptr, 0, 0, st)) return rc;
     return PYGHO_OK;
   }
-  if (!x || !w || !gy || !workspace) { set_error("null pointer"); return PYGHO_ERR_INVALID; }
-  const int es = la_size(dtype);
-  char* base = reinterpret_cast<char*>(workspace);
-  // (`out`: dz's place, aligned by its own rule; gx joins the condition because dX is stored in the same launch)
-  LsArgs fa = la_stream_args(x, x_ld, w, w_ld, bias, bias_dtype, g, h, norm_dtype, gy, gy_ld, base, m_cap, k, n, eps, act, dtype);
-  if (gx && !(k % 16 == 0 && la_aligned(gx, k, es, 16))) fa.vec &= 1;
-  fa.m_dev = m_dev;
-  const LaSpace sp = la_space(m_cap, k, n, norm, act, dtype, fa.vec == 3);
+  if (!x || !w || !gy) { set_error("null pointer"); return PYGHO_ERR_INVALID; }
+  const int vec = la_vec_bwd(gx, x, x_ld, gy, gy_ld, k, n, dtype);
+  const LaSpace sp = la_space(m_cap, k, n, norm, act, dtype, LaAsk{gx != nullptr, gw != nullptr, gb != nullptr, vec == 3});
+  if (sp.total > 0 && !workspace) { set_error("null pointer"); return PYGHO_ERR_INVALID; }
   if (workspace_bytes < (size_t)sp.total || (uintptr_t)workspace % 16 != 0) { set_error("linear_act_bwd: workspace too small or not 16-byte aligned"); return PYGHO_ERR_INVALID; }
   if (pygho_linear_act_keeps(k, n, norm, act, dtype) != 0 && !z) { set_error("linear_act_bwd: the kept pre-activation is missing"); return PYGHO_ERR_INVALID; }
+  char* base = reinterpret_cast<char*>(workspace);
+  LsArgs fa = la_stream_args(x, x_ld, w, w_ld, bias, bias_dtype, g, h, norm_dtype, gy, gy_ld, base, m_cap, k, n, eps, act, dtype);
+  fa.vec = vec;
+  fa.m_dev = m_dev;
   if (sp.fused) {
     fa.out = nullptr;
     fa.gx = gx;
@@ -203,7 +222,8 @@ extern "C" int pygho_linear_act_bwd(void* gx, void* gw, int gw_dtype, void* gb, 
     int used = 0;
     if (sp.stream) {
       fa.slabs = slabs; fa.slab_stride = stride;
-      if (gx && la_type(dtype, [&](auto ops) { return ops.stream_lds(k, n, sp.nsum, true, false) <= kLsLds; })) {
+      if (!sp.dz) fa.out = nullptr;
+      if (sp.gx_here) {
         fa.gx = gx;
         have_gx = true;
       }
@@ -241,17 +261,17 @@ extern "C" int pygho_linear_act_bwd(void* gx, void* gw, int gw_dtype, void* gb, 
     }
   }
   const bool db_here = gb && !sp.own_dz;                      // dz is gy itself: its column sums come with dW
-  if (gw || db_here) {
+  if (sp.dw_k) {
     LaArgs a{};
     a.a = {dz, dz_ld};
     a.b = {x, x_ld};
-    a.m = n; a.n = k; a.k = m_cap; a.dev = m_dev;
+    a.m = n; a.n = sp.dw_k; a.k = m_cap; a.dev = m_dev;
     a.slabs = reinterpret_cast<float*>(base + sp.dz + sp.z + sp.sums);
-    a.slab_stride = la_pad4(n * k + n);
-    a.splits = (int)la_dw_slabs(m_cap, k, n);
+    a.slab_stride = la_pad4(n * sp.dw_k + n);
+    a.splits = (int)la_dw_slabs(m_cap, sp.dw_k, n);
     a.want_sums = db_here;
     if (int rc = la_type(dtype, [&](auto ops) { return ops.tile_dw(a, st); })) return rc;
-    const FoldOut o{{gw, db_here ? gb : nullptr, nullptr, nullptr}, {n * k, db_here ? n : 0, 0, 0}, {gw_dtype, gb_dtype, 0, 0}};
+    const FoldOut o{{gw, db_here ? gb : nullptr, nullptr, nullptr}, {n * sp.dw_k, db_here ? n : 0, 0, 0}, {gw_dtype, gb_dtype, 0, 0}};
     if (int rc = fold_launch(o, a.slabs, a.splits, a.slab_stride, st)) return rc;
   }
   return PYGHO_OK;

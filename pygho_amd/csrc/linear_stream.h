@@ -25,7 +25,7 @@ struct LsArgs {
   const void* w; int64_t w_ld; int w_trans;                   // w_trans: w is stored [k][n] (the W of dz . W)
   const void* bias; int bias_dtype; const void* g; const void* h; int norm_dtype;
   const void* r; int64_t r_ld;                                // residual (forward) / output gradient (backward)
-  void* out; int out_f32;                                     // y / dz; out_f32 (LS_ACT): f32 values as they are
+  void* out; int out_f32;                                     // y / dz (nullable: no later launch reads it); out_f32 (LS_ACT): f32 values as they are
   void* gx;                                                   // backward, nullable: dX (rows of k)
   float* slabs; int64_t slab_stride;                          // backward: LS_DACT [gb], LS_DNORM [gg | gh | gb]
   int64_t m; const int32_t* m_dev; int k; int n; float eps; int act;
@@ -153,7 +153,7 @@ template <typename T, int NB> struct LsGeom {
   static constexpr int param_bytes = 4 * NP * 4;
 };
 // the fused weight gradient: workgroups of 4 wavefronts, two per CU, each at its own place in the sequence of phases between its barriers
-constexpr int kLsDwWaves = 4;
+constexpr int kLsDwWaves = 4, kLsDwGrid = 256 * 2;
 
 // VEC & 1: k is a whole number of 64-byte steps and x's rows allow 16-byte accesses.  VEC & 2: n is a whole number of 16 channels and the rows of r, out
 // and gx are on 16-byte boundaries (k of 16, with gx).  A block's rows then are one uniform base address, one 32-bit offset per lane and
@@ -509,7 +509,7 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC, size
           for (int i = 0; i < NB * 4; ++i) t[i] = d[i / 4][i % 4];
           add_rows(NSUM ? NSUM - 1 : 0, t);
         }
-        if constexpr (!DW) store_rows(reinterpret_cast<T*>(a.out), d, N);
+        if constexpr (!DW) { if (a.out) store_rows(reinterpret_cast<T*>(a.out), d, N); }
         if constexpr (!DX && AHEAD) load_r(blk + stride);
         if constexpr (DX) {
           // dz as the operand of dz . W and dz^T x: step s of n = this lane's registers 2 s, 2 s + 1 (16-bit) or s (f32).  16-bit rows: dz is rounded to
@@ -681,9 +681,9 @@ template <typename T, int NB, int EPI, bool DX, int VEC, bool DW = false> static
   int per_cu = std::min(WPS, std::max(1, 160 * 1024 / lds));
   while (WPS * 4 % per_cu != 0) --per_cu;
   int waves = WPS * 4 / per_cu;
-  if (DW) { waves = kLsDwWaves; per_cu = 2; }
+  if (DW) waves = kLsDwWaves;
   else if (NSUM == 0 && blocks < 256 * 4 * WPS) waves = std::min(waves, 4);
-  const int grid = (int)std::min<int64_t>(ceil_div(blocks, waves), 256 * per_cu);
+  const int grid = (int)std::min<int64_t>(ceil_div(blocks, waves), DW ? kLsDwGrid : 256 * per_cu);
   if (n_slabs) *n_slabs = grid;
   hipLaunchKernelGGL((linear_stream_kernel<T, NB, EPI, DX, VEC, DW>), dim3(grid), dim3(waves * kWave), lds, st, a);
   return check_launch("linear_stream");

@@ -206,7 +206,8 @@ class _LinearAct(torch.autograd.Function):
         gb, gb_ptr, gb_code = _grad(need_b, n, b_dtype, dev)
         gg, gg_ptr, gg_code = _grad(need_g, n, g_dtype, dev)
         gh, gh_ptr, gh_code = _grad(need_h, n, h_dtype, dev)
-        nbytes = int(lib().pygho_linear_act_bwd_workspace(m, k, n, int(normed), ROW_ACT_CODE[act], code))
+        nbytes = int(lib().pygho_linear_act_bwd_workspace_for(ptr(gx), need_w, need_b, ptr(x2), x_ld, ptr(gy2), gy_ld, m, k, n, int(normed),
+                                                              ROW_ACT_CODE[act], code))
         ws, count = _workspace(nbytes, dev), _device_rows(x_shape)
         check(lib().pygho_linear_act_bwd(ptr(gx), gw_ptr, gw_code, gb_ptr, gb_code, gg_ptr, gg_code, gh_ptr, gh_code, ptr(z), ptr(x2), x_ld, ptr(w),
                                          w_ld, ptr(b), bdt, int(normed), ptr(g), ptr(h), pdt, float(eps), ptr(gy2), gy_ld, m, ptr(count),

@@ -300,3 +300,54 @@ def test_fused_mlp_on_rows_far_apart(dev):
     t = x.clone().requires_grad_(True)
     got, want = (torch.autograd.grad(m(t), [t, *m.parameters()], g) for g in (gfar, gy))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---- only what is asked for ----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("norm", [0, 1])
+@pytest.mark.parametrize("k,n", [(128, 128), (96, 112), (384, 128), (100, 36), (256, 256), (40, 300), (512, 512)])
+def test_the_workspace_of_a_call_holds_it(dev, dtype, norm, k, n):
+    """the C entry with just the bytes that the query for this call names, for every subset of gradients and both activations' plans: nothing is
+    written behind them, and the values are those of the call with every gradient in the largest workspace"""
+    import itertools
+    from pygho_amd import _ops
+    from pygho_amd._native import DTYPE_CODE, check, lib, ptr, stream_ptr
+    gen = torch.Generator(device=dev).manual_seed(k + n)
+    m, code, guard = 777, DTYPE_CODE[dtype], 1 << 14
+    x, w, b, g, h, gy = (torch.randn(s, generator=gen, device=dev).div_(4).to(dtype) for s in ((m, k), (n, k), (n,), (n,), (n,), (m, n)))
+    names = ("gx", "gw", "gb") + (("gg", "gh") if norm else ())
+    for act in (_ops.ROW_ACT_CODE["none"], _ops.ROW_ACT_CODE["silu"]):
+        keeps = int(lib().pygho_linear_act_keeps(k, n, norm, act, code))
+        y, z = torch.empty_like(gy), torch.empty((m, n), dtype=torch.float32 if keeps == 2 else dtype, device=dev)
+        check(lib().pygho_linear_act(ptr(y), ptr(z), ptr(x), k, ptr(w), k, ptr(b), code, norm, ptr(g), ptr(h), code, 1e-5, None, 0, m, k, n, act, code,
+                                     stream_ptr(dev)), "linear_act")
+
+        def backward(ask, nbytes):
+            out = {name: torch.full(s, 7.0, dtype=dtype, device=dev) for name, s in (("gx", (m, k)), ("gw", (n, k)), ("gb", (n,)), ("gg", (n,)), ("gh", (n,)))
+                   if name in ask}
+            if nbytes is None:
+                nbytes = int(lib().pygho_linear_act_bwd_workspace_for(ptr(out.get("gx")), "gw" in ask, "gb" in ask, ptr(x), k, ptr(gy), n, m, k, n, norm,
+                                                                      act, code))
+                assert nbytes <= int(lib().pygho_linear_act_bwd_workspace(m, k, n, norm, act, code))
+            ws = torch.full((nbytes + guard,), 0xA5, dtype=torch.uint8, device=dev)
+            p = {name: ptr(out.get(name)) for name in ("gx", "gw", "gb", "gg", "gh")}
+            check(lib().pygho_linear_act_bwd(p["gx"], p["gw"], code, p["gb"], code, p["gg"], code, p["gh"], code, ptr(z) if keeps else None, ptr(x), k, ptr(w), k,
+                                             ptr(b), code, norm, ptr(g), ptr(h), code, 1e-5, ptr(gy), n, m, None, k, n, act, code, ptr(ws), nbytes,
+                                             stream_ptr(dev)), "linear_act_bwd")
+            assert bool((ws[nbytes:] == 0xA5).all()), (act, ask)
+            return out
+        want = backward(names, int(lib().pygho_linear_act_bwd_workspace(m, k, n, norm, act, code)))
+        for pick in itertools.product((False, True), repeat=len(names)):
+            ask = [name for name, f in zip(names, pick) if f]
+            got = backward(ask, None)
+            for name in ask:
+                # dX without an activation or a norm is gy . W in either of two launches: the same n products in another order, each off by at most
+                # n 2^-24 of their absolute sum and rounded once (two of 128 x 128 bf16 values differ in the last bit).  With one: the same order
+                if name == "gx" and not norm and act == _ops.ROW_ACT_CODE["none"]:
+                    v = want[name].double()
+                    same(got[name], v, v.abs() * 2 * HALF[dtype] + 2 * n * 2.0 ** -24 * (gy.double().abs() @ w.double().abs()) + TINY[dtype], f"{ask} gx")
+                elif name == "gx":
+                    assert torch.equal(got[name], want[name]), (act, ask)
+                else:                                           # other slabs: the rows in another order, chains of at most 256 sums of m terms below 1 on average
+                    v = want[name].double()
+                    same(got[name], v, v.abs() * 2 * HALF[dtype] + 256 * 2.0 ** -24 * m, f"{act} {ask} {name}")
