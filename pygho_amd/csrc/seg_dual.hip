@@ -61,9 +61,8 @@ template <typename T> __device__ __forceinline__ du_u4_t du_pack(const float (&v
   return du_u4_t{u.x, u.y, u.z, u.w};
 }
 
-// two channels of a 16-bit word as a float pair: the products and sums below are written on PAIRS so that they issue as packed f32
-// instructions (v_pk_fma_f32: two exact-product fmas per lane and issue slot); the kernel is bound by vector issue (PMC: 440 vector
-// instructions per chunk and wavefront, 60 % of them conversions of 16-bit rows)
+// two channels of a 16-bit word as a float pair; a pair's product or sum is two scalar f32 instructions (build.py switches the packed forms off:
+// one issue slot for both, but not safe on these cards).  The kernel is bound by vector issue, most of it conversions of 16-bit rows and these
 typedef float du_f2_t __attribute__((ext_vector_type(2)));
 template <typename T> __device__ __forceinline__ du_f2_t du_pair(uint32_t w);
 template <> __device__ __forceinline__ du_f2_t du_pair<bf16>(uint32_t w) { return du_f2_t{__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)}; }
@@ -76,7 +75,7 @@ __device__ __forceinline__ du_f2_t du_fma(du_f2_t a, du_f2_t b, du_f2_t c) { ret
 
 // TG ("table gradient"): the second operand is a lookup into a table whose looked-up rows are all < kDuTgRows (bond types): the by-edge
 // half does not form the per-edge gradient at all -- every lane group accumulates the gradient of the TABLE rows in registers
-// (kDuTgRows x 8 channels: g[a] * H[c] routed by a 0 / 1 factor per table row), the lane groups of a wavefront are summed by shuffles
+// (kDuTgRows x 8 channels: g[a] * H[c] added to the message's row under a branch per table row), the lane groups of a wavefront are summed by shuffles
 // once at the end, and every workgroup writes one f32 slab (`tg_out`, folded by pygho_sum_blocks).  No edge accumulators in LDS (8.3
 // instead of 19.8 KB per wavefront: three workgroups per CU instead of two), no read-modify-write per message, no edge rows written
 // and read back (0.2 GB per launch), no table_grad launch behind it.  The table gradient is then the f32 sum of exact products --
@@ -348,13 +347,14 @@ __global__ __launch_bounds__(TG ? 256 : 512, TG ? 3 : 1) void seg_dual_kernel(
         du_f2_t pr[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) pr[i] = du_pair<T>(gv[t][i]) * du_pair<T>(xv[t][i]);     // exact products
+        // (a branch per table row: a 0 / 1 factor per row takes 32 products per message whatever rows there are -- 10.70 ms per training step for
+        // 10.63 -- and carries an infinity into every row as 0 * inf)
 #pragma unroll
-        for (int tt = 0; tt < kDuTgRows; ++tt) {
-          const float sel = (valid && look == (uint32_t)tt) ? 1.f : 0.f;
-          const du_f2_t s2 = du_f2_t{sel, sel};
+        for (int tt = 0; tt < kDuTgRows; ++tt)
+          if (valid && look == (uint32_t)tt) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) tg[tt][i] = du_fma(pr[i], s2, tg[tt][i]);
-        }
+            for (int i = 0; i < 4; ++i) tg[tt][i] += pr[i];
+          }
       }
     }
   };
