@@ -11,8 +11,8 @@
 //   * channel sums (gg, gh, gb) are taken from the unrounded f32 values, over a block's 16 rows by lane exchanges (ls_row_sums).
 // Block b of the rows belongs to wavefront b % (all wavefronts), so sums depend on the true row count only (see layer_norm.hip).
 // Measured, bf16 with a norm and a residual, 1.83 M x 128 -> 128: forward 265 us (1.41 GB: 5.3 TB/s, what a copy reaches), whole gradient in one
-// launch 510 .. 545 us (1.41 GB; vector issue 63 %, matrix cores 18 % of the cycles: bound by instructions at two wavefronts per SIMD, a quarter
-// of them the three row sums) + fold 16
+// launch 475 .. 525 us (1.41 GB; vector issue 63 %, matrix cores 18 % of the cycles: bound by instructions at two wavefronts per SIMD, a quarter
+// of them the three row sums; bank conflicts are 47 % of the LDS-active cycles, waits for LDS 11 % of the wavefronts') + fold 16
 #pragma once
 #include "linear_tile.h"
 
