@@ -875,9 +875,11 @@ int pygho_layer_norm_act_bwd(void* gx, void* gweight, int gweight_dtype, void* g
  *   z = x (m, k) . w (n, k)^T + bias,    y = act(z) + residual,    with `norm`: y = act(xh g + h) + residual, xh the layer norm of z over n
  *   (bias / g / h / residual nullable = 0 / 1 / 0 / 0; w in the rows' type).
  * z: the pre-activation, (m, n).  pygho_linear_act_keeps says whether the backward of this shape reads it: 0 no (z is formed again from x; pass
- *   NULL), 1 yes, in the rows' type (a finite value beyond it as its largest; NULL in a forward that no backward follows), 2 yes, in f32 (the
- *   forward itself needs the buffer).
+ *   NULL), 1 yes, in the rows' type, or in f32 where both calls have PYGHO_ROW_Z_F32 in `act` (NULL in a forward that no backward follows), 2 yes,
+ *   in f32 (the forward itself needs the buffer).  In a 16-bit type the activation's slope is that of the rounded z (a finite value beyond the type
+ *   is kept as its largest); f32 gives the slope that the other shapes have.
  * backward: dz = the gradient of z,   gx = dz . w (nullable),   gw = dz^T . x,   gb = sum_m dz,   gg / gh as gweight / gbias above. */
+enum { PYGHO_ROW_Z_F32 = 0x100 };
 int pygho_linear_act_keeps(int64_t k, int64_t n, int norm, int act, int dtype);
 int pygho_linear_act(void* y, void* z, const void* x, int64_t x_ld, const void* w, int64_t w_ld, const void* bias, int bias_dtype, int norm,
                      const void* g, const void* h, int norm_dtype, double eps, const void* residual, int64_t residual_ld, int64_t m, int64_t k,

@@ -137,8 +137,8 @@ static int la_vec_bwd(const void* gx, const void* x, int64_t x_ld, const void* g
 
 using namespace pygho;
 
-// what the forward keeps for the backward besides x: 0 nothing, 1 the pre-activation in the rows' type, 2 the pre-activation in f32 (needed by the
-// forward itself as well)
+// what the forward keeps for the backward besides x: 0 nothing, 1 the pre-activation in the rows' type or in f32 (PYGHO_ROW_Z_F32), 2 the
+// pre-activation in f32 (needed by the forward itself as well)
 extern "C" int pygho_linear_act_keeps(int64_t k, int64_t n, int norm, int act, int dtype) {
   if (k <= 0 || n <= 0 || !ro_float(dtype) || la_form(k, n, norm, dtype) != FORM_TILE) return 0;
   return norm ? 2 : act != kActNone ? 1 : 0;
@@ -147,6 +147,8 @@ extern "C" int pygho_linear_act_keeps(int64_t k, int64_t n, int norm, int act, i
 extern "C" int pygho_linear_act(void* y, void* z, const void* x, int64_t x_ld, const void* w, int64_t w_ld, const void* bias, int bias_dtype, int norm,
                                 const void* g, const void* h, int norm_dtype, double eps, const void* residual, int64_t residual_ld, int64_t m,
                                 int64_t k, int64_t n, int act, int dtype, void* stream) {
+  const int z_f32 = (act & PYGHO_ROW_Z_F32) != 0;
+  act &= ~PYGHO_ROW_Z_F32;
   if (int rc = la_check("linear_act", m, k, n, eps, act, dtype)) return rc;
   if (int rc = la_param_check("linear_act", bias, bias_dtype, dtype)) return rc;
   if (g || h) { if (int rc = la_param_check("linear_act", g ? g : h, norm_dtype, dtype)) return rc; }
@@ -156,7 +158,7 @@ extern "C" int pygho_linear_act(void* y, void* z, const void* x, int64_t x_ld, c
   hipStream_t st = (hipStream_t)stream;
   if (const int form = la_form(k, n, norm, dtype); form != FORM_TILE)
     return la_forward(la_stream_args(x, x_ld, w, w_ld, bias, bias_dtype, g, h, norm_dtype, residual, residual_ld, y, m, k, n, eps, act, dtype), form, norm, dtype, st);
-  if (!norm) return la_tile_act(x, x_ld, w, w_ld, bias, bias_dtype, residual, residual_ld, y, z, 0, m, nullptr, k, n, act, dtype, st);
+  if (!norm) return la_tile_act(x, x_ld, w, w_ld, bias, bias_dtype, residual, residual_ld, y, z, z_f32, m, nullptr, k, n, act, dtype, st);
   if (!z) { set_error("linear_act: this norm needs the pre-activation's buffer (pygho_linear_act_keeps)"); return PYGHO_ERR_INVALID; }
   if (int rc = la_tile_act(x, x_ld, w, w_ld, bias, bias_dtype, nullptr, 0, nullptr, z, 1, m, nullptr, k, n, kActNone, dtype, st)) return rc;
   return ln_fwd_launch(y, z, n, g, h, norm_dtype, residual, residual_ld, m, n, (float)eps, act, dtype, PYGHO_F32, st);
@@ -178,6 +180,8 @@ extern "C" int pygho_linear_act_bwd(void* gx, void* gw, int gw_dtype, void* gb, 
                                     int norm, const void* g, const void* h, int norm_dtype, double eps, const void* gy, int64_t gy_ld,
                                     int64_t m_cap, const int32_t* m_dev, int64_t k, int64_t n, int act, int dtype, void* workspace,
                                     size_t workspace_bytes, void* stream) {
+  const bool z_f32 = (act & PYGHO_ROW_Z_F32) != 0;
+  act &= ~PYGHO_ROW_Z_F32;
   if (int rc = la_check("linear_act_bwd", m_cap, k, n, eps, act, dtype)) return rc;
   if (int rc = la_param_check("linear_act_bwd", bias, bias_dtype, dtype)) return rc;
   if (g || h) { if (int rc = la_param_check("linear_act_bwd", g ? g : h, norm_dtype, dtype)) return rc; }
@@ -237,7 +241,7 @@ extern "C" int pygho_linear_act_bwd(void* gx, void* gw, int gw_dtype, void* gb, 
         z = base + sp.dz;
       }
       if (int rc = ln_bwd_launch(own, slabs, &stride, &used, sp.nsum, z, n, gy, gy_ld, g, h, norm_dtype, m_cap, m_dev, n, (float)eps, act, dtype,
-                                 norm || sp.z ? PYGHO_F32 : dtype, st)) return rc;
+                                 norm || sp.z || z_f32 ? PYGHO_F32 : dtype, st)) return rc;
     }
     dz = own;
     dz_ld = n;

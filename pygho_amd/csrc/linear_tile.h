@@ -174,9 +174,8 @@ template <typename T> __device__ __forceinline__ void la_store4(T* p, int left, 
   }
 }
 
-// A pre-activation on its way into 16-bit storage.  A finite one beyond the type's range becomes the type's largest value: as an infinity it would make
-// silu's slope inf * 0 = NaN, where the forms that keep z in f32 give 0 or 1 (f16 reaches 65504).  Infinities and NaN stay what they are.
-// The slope of a gradient is then taken from the rounded z, as where nn.Linear keeps it; f32 storage costs the forward 87 us for 66 (65536 x 512 -> 512)
+// A pre-activation on its way into 16-bit storage (a caller's choice: rowops.py keeps it in f32).  A finite one beyond the type's range becomes the
+// type's largest value: as an infinity it would make silu's slope inf * 0 = NaN, where f32 gives 0 or 1 (f16 reaches 65504).  Infinities and NaN stay
 template <typename T> __device__ __forceinline__ float la_in_range(float v) {
   constexpr float most = std::is_same<T, f16>::value ? 65504.f : std::is_same<T, bf16>::value ? 3.38953139e38f : 3.40282347e38f;
   return fabsf(v) <= 3.40282347e38f ? fminf(fmaxf(v, -most), most) : v;

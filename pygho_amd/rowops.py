@@ -25,6 +25,7 @@ from .blocks import param_as
 from .plans import dyn_rows
 
 ROW_ACT_CODE = {"none": 0, "relu": 1, "silu": 2, "elu": 3}      # enum pygho_row_act
+_Z_F32 = 0x100                                                   # PYGHO_ROW_Z_F32
 _ROW_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
@@ -182,9 +183,11 @@ class _LinearAct(torch.autograd.Function):
         z = None
         # (`training`: the caller's grad mode.  In here it is always off, and needs_input_grad says what the inputs ask for in either mode)
         if keeps == 2 or (keeps == 1 and training and any(ctx.needs_input_grad[:5])):
-            z = torch.empty((m, n), dtype=torch.float32 if keeps == 2 else dt, device=dev)
+            # in f32 for 16-bit rows too: the slope is then that of the unrounded z, as in the forms that form it again (a z rounded to bf16 moves silu's
+            # slope by up to 2^-8).  Training bf16 65536 x 512 -> 512 361 us, with 16 bits 354; 300 -> 300 368, 342
+            z = torch.empty((m, n), dtype=torch.float32, device=dev)
         check(lib().pygho_linear_act(ptr(y), ptr(z), ptr(x2), x_ld, ptr(w), w_ld, ptr(b), bdt, int(normed), ptr(gg), ptr(hh), pdt, float(eps),
-                                     ptr(r2), r_ld, m, k, n, ROW_ACT_CODE[act], code, stream_ptr(dev)), "linear_act")
+                                     ptr(r2), r_ld, m, k, n, ROW_ACT_CODE[act] | _Z_F32, code, stream_ptr(dev)), "linear_act")
         ctx.save_for_backward(x2, w, b, z, gg, hh)
         ctx.meta = (x_ld, w_ld, bdt, pdt, eps, act, normed, x.shape, weight.dtype, *(None if t is None else t.dtype for t in (bias, g, h)))
         return y
@@ -211,7 +214,7 @@ class _LinearAct(torch.autograd.Function):
         ws, count = _workspace(nbytes, dev), _device_rows(x_shape)
         check(lib().pygho_linear_act_bwd(ptr(gx), gw_ptr, gw_code, gb_ptr, gb_code, gg_ptr, gg_code, gh_ptr, gh_code, ptr(z), ptr(x2), x_ld, ptr(w),
                                          w_ld, ptr(b), bdt, int(normed), ptr(g), ptr(h), pdt, float(eps), ptr(gy2), gy_ld, m, ptr(count),
-                                         k, n, ROW_ACT_CODE[act], code, ptr(ws), nbytes, stream_ptr(dev)), "linear_act_bwd")
+                                         k, n, ROW_ACT_CODE[act] | _Z_F32, code, ptr(ws), nbytes, stream_ptr(dev)), "linear_act_bwd")
         return gx, gw, gb, gg, gh, res, None, None, None, None
 
 

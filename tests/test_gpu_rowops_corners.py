@@ -102,6 +102,46 @@ def test_f16_pre_activations_beyond_the_type(dev, k, n, act):
         assert bool(torch.isnan(gx[3]).all()) and bool(torch.isfinite(gx[:3]).all()) and bool(torch.isfinite(gx[4:]).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ["silu", "elu"])
+@pytest.mark.parametrize("m,k,n", [(1, 244, 344), (1, 512, 512), (2, 300, 300), (1, 256, 256), (1, 128, 128), (3, 600, 100), (1, 40, 700)])
+def test_the_slope_is_that_of_the_unrounded_pre_activation(dev, m, k, n, act, dtype):
+    """few rows, so that no average hides it: gx and gw within one rounding of dz and one of the result (the bounds of `block_reference`), in the forms
+    that keep z as in those that form it again.  A z rounded to bf16 moves silu's slope by up to 2^-8"""
+    from test_gpu_rowops import block_check, grid_values
+    gen = torch.Generator(device=dev).manual_seed(m + k + n)
+    x = grid_values(gen, (m, k), dev, 1.0).add_(0.25).to(dtype)
+    w = (torch.rand(n, k, generator=gen, device=dev) * 2 - 1).div_(k ** 0.5).to(dtype)
+    gy = grid_values(gen, (m, n), dev, 1.0).to(dtype)
+    block_check(False, x, w, None, None, None, 0.0, act, None, gy, f"{m} x {k} -> {n}")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_a_caller_of_the_c_entry_may_keep_z_in_the_rows_type(dev, dtype):
+    """both storages of z through the C entry, with a z beyond f16: values and slopes of an exact product"""
+    from pygho_amd import _ops
+    from pygho_amd._native import DTYPE_CODE, check, lib, ptr, stream_ptr
+    m, k, n, code, silu = 40, 512, 512, DTYPE_CODE[dtype], _ops.ROW_ACT_CODE["silu"]
+    sign = torch.where(torch.arange(n, device=dev) % 2 == 0, 1.0, -1.0)
+    x, w = torch.full((m, k), 1024.0, device=dev, dtype=dtype), (0.5 * sign[:, None]).expand(n, k).contiguous().to(dtype)
+    gy = (torch.arange(m * n, device=dev) % 3 - 1).reshape(m, n).to(dtype)
+    want = ((gy.double() * (sign > 0)) @ w.double()).to(dtype)
+    assert int(lib().pygho_linear_act_keeps(k, n, 0, silu, code)) == 1
+    nbytes = int(lib().pygho_linear_act_bwd_workspace(m, k, n, 0, silu, code))
+    for flag, zt in ((0, dtype), (0x100, torch.float32)):
+        y, gx, ws = torch.empty_like(gy), torch.empty_like(x), torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        z = torch.full((m + 1, n), 7.0, dtype=zt, device=dev)
+        check(lib().pygho_linear_act(ptr(y), ptr(z), ptr(x), k, ptr(w), k, None, 0, 0, None, None, 0, 0.0, None, 0, m, k, n, silu | flag, code, stream_ptr(dev)),
+              "linear_act")
+        full = 1024.0 * 0.5 * k * sign
+        if zt == torch.float16:
+            full = full.clamp(-65504.0, 65504.0)
+        assert torch.equal(z[:m].double(), full.double().expand(m, n)) and bool((z[m] == 7.0).all())
+        check(lib().pygho_linear_act_bwd(ptr(gx), None, 0, None, 0, None, 0, None, 0, ptr(z), ptr(x), k, ptr(w), k, None, 0, 0, None, None, 0, 0.0, ptr(gy), n, m,
+                                         None, k, n, silu | flag, code, ptr(ws), nbytes, stream_ptr(dev)), "linear_act_bwd")
+        assert torch.equal(gx, want), (flag, zt)
+
+
 # ---- infinities in the last row ----------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("k,n", [(128, 128), (64, 64), (96, 112), (100, 36), (384, 128), (256, 256), (512, 512)])

@@ -60,3 +60,16 @@ def test_a_call_asks_for_the_workspace_it_uses():
     rc = lib().pygho_linear_act_bwd(one, None, 0, None, 0, None, 0, None, 0, None, one, 128, one, 128, None, 0, 1, None, None, bf16, 1e-5, one, 128, 5000,
                                     None, 128, 128, 2, bf16, None, 0, None)
     assert rc == 1 and b"null" in lib().pygho_last_error()
+
+
+def test_the_flag_of_an_f32_pre_activation_leaves_the_checks_as_they_are():
+    import ctypes
+    from pygho_amd._native import lib
+    one = ctypes.c_void_p(16)                                            # never dereferenced: the checks fail first
+
+    def fwd(act, m=5, dt=1):
+        return lib().pygho_linear_act(one, one, one, 64, one, 64, None, 0, 0, None, None, 1, 0.0, None, 0, m, 64, 64, act, dt, None)
+    assert fwd(0x102, m=0) == 0 and fwd(0x104) == 1 and fwd(0x200) == 1 and fwd(0x102, dt=3) == 2
+    rc = lib().pygho_linear_act_bwd(one, None, 0, None, 0, None, 0, None, 0, None, one, 512, one, 512, None, 0, 0, None, None, 1, 0.0, one, 512, 5, None, 512, 512,
+                                    0x102, 1, one, 1 << 30, None)
+    assert rc == 1 and b"missing" in lib().pygho_last_error()
