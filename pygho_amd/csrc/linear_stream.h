@@ -349,9 +349,10 @@ __global__ __launch_bounds__(DW ? kLsDwWaves * kWave : ls_wps(NB, EPI, VEC, size
         if (kc + 1 < nk) load_x(blk, kc + 1, xn);
         else load_x(min(blk + stride, n_blocks - 1), 0, xn);
       }
+      // (dz = gy without an activation: the fused gradient has no use for z)
 #pragma unroll
       for (int s = 0; s < KC; ++s) {
-        if (kc * KC + s < KS) {
+        if (kc * KC + s < KS && !(DW && EPI == LS_DACT && a.act == kActNone)) {
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) {
             const uint4 fa = *reinterpret_cast<const uint4*>(lds_w + (nb * 16 + r16) * pitch + (kc * KC + s) * 64 + q * 16);
